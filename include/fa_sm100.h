@@ -214,6 +214,121 @@ int fa_bwd_dkdv(const fa_params* p, void* stream); /* _attn_bwd_dkdv       FA:33
 int fa_bwd_dq(const fa_params* p, void* stream);   /* _attn_bwd_dq         FA:538-646 */
 
 /*
+ * ---- Paged key / value cache: attention of one new token a sequence, and the upkeep of the cache -------------------------
+ * No counterpart in the reference, which has no cache.
+ *
+ * A cache is num_pages pages of page_size tokens of Hkv heads: element (page, token, head, d) of k_cache and v_cache lies at
+ * page * stride[0] + token * stride[1] + head * stride[2] + d.  Row b of block_table names the pages of sequence b in order;
+ * the key at position n of it is token n % page_size of page block_table[b][n / page_size].  Entries behind the last page
+ * of a sequence are not read.
+ */
+
+/*
+ * Attention of one new token: q and o are (B, H, D), head h reads key head h / (H / Hkv), and sequence b has the keys at
+ * positions 0 .. seq_lens[b] - 1 (the new token's own key is written before).  o = softmax(q.k^T * sm_scale + bias) . v in one
+ * pass over the pages, split over their length and joined in a fixed order: the same call gives the same bits.
+ *   bias: (B, H, width * page_size), kinds as in fa_params, at any naturally aligned address with any strides over B and H
+ *     (0 included).  A key that a mask or a bias of -inf leaves out takes no part, whatever its key and value hold.
+ *   A length below 0 counts as 0, one above width * page_size as that; keys on a page outside 0 .. num_pages - 1 take no part.
+ *   A row without any key: 0.
+ * Alignment: q, k_cache, v_cache, o and their strides * 2 bytes are multiples of 16.
+ */
+typedef struct fa_paged_params {
+  uint32_t struct_size; /* sizeof(fa_paged_params), checked against the library */
+  int32_t device;
+  int32_t B, H, Hkv, D;
+  int32_t page_size;
+  int32_t width;     /* entries of a row of block_table */
+  int32_t num_pages; /* of the cache */
+  int32_t dtype;     /* fa_dtype of q, k_cache, v_cache, o */
+  int32_t bias_kind; /* fa_bias_kind */
+  float sm_scale;
+
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  const int32_t* block_table; /* (B, width), rows table_stride elements apart */
+  const int32_t* seq_lens;    /* (B) */
+  const void* bias;
+
+  int64_t q_stride[2]; /* B, H */
+  int64_t o_stride[2];
+  int64_t k_stride[3]; /* page, token, head */
+  int64_t v_stride[3];
+  int64_t bias_stride[2]; /* B, H */
+  int64_t table_stride;
+} fa_paged_params;
+
+/*
+ * Scratch of a call, a function of the sizes alone (0: none is needed): 16-byte aligned device memory, contents unspecified
+ * before and after, not shared by calls that may overlap on the GPU.
+ */
+uint64_t fa_paged_workspace_bytes(const fa_paged_params* p);
+int fa_paged_fwd(const fa_paged_params* p, void* workspace, uint64_t bytes, void* stream);
+
+/*
+ * Rows into the cache: k and v of token t, (T, Hkv, D) of 16-bit elements, to slot s = slots[t], token s % page_size of page
+ * s / page_size.  A slot below 0 or behind the cache: that token is not written.  The slots of a call are different; k and v do
+ * not overlap the cache.  Alignment as above; the strides of the cache are positive.
+ */
+typedef struct fa_kv_write_params {
+  uint32_t struct_size;
+  int32_t device;
+  int32_t T, Hkv, D;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t reserved;
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slots; /* (T) */
+  int64_t k_stride[2];  /* token, head */
+  int64_t v_stride[2];
+  int64_t k_cache_stride[3]; /* page, token, head */
+  int64_t v_cache_stride[3];
+} fa_kv_write_params;
+int fa_kv_write(const fa_kv_write_params* p, void* stream);
+
+/*
+ * Pages and slots for new tokens, and pages given back; the free pages are a stack of which free_pages[0 .. *count - 1] are free.
+ *
+ * fa_kv_extend: request b holds lens[b] tokens and brings change[b] more (below 0 counts as 0); its tokens are rows
+ *   off(b) .. off(b) + change[b] - 1 of the call, off the running sum.  It needs the pages that its old ones have no room for.
+ *   Requests are served in order: one that does not fit its row of the table (width * page_size tokens) or whose tokens reach
+ *   beyond T gets nothing, and so does each that needs pages from the first on that finds too few.  A served request's new
+ *   pages come off the top of the stack into block_table, lens_out[b] is its new length, and slots[row] the slot of each of its
+ *   tokens; all other slots are -1, and lens_out[b] of a request that got nothing is lens[b].  count_out: pages left.
+ * fa_kv_release: the pages of each request b with finished[b] != 0 go back on the stack, requests and pages in order, and
+ *   lens_out[b] is 0 (else lens[b]).  Pages beyond the stack's capacity are dropped.  block_table is only read.
+ *
+ * lens_out may be lens, and count_out may be count.
+ */
+typedef struct fa_kv_table_params {
+  uint32_t struct_size;
+  int32_t device;
+  int32_t B;
+  int32_t width;
+  int32_t page_size;
+  int32_t capacity; /* entries of free_pages */
+  int32_t T;        /* extend: entries of slots */
+  int32_t reserved;
+  int32_t* block_table; /* (B, width) */
+  const int32_t* lens;  /* (B) */
+  const int32_t* change;     /* extend: (B) */
+  const uint8_t* finished;   /* release: (B) */
+  int32_t* free_pages;  /* (capacity) */
+  const int32_t* count; /* (1) */
+  int32_t* lens_out;    /* (B) */
+  int32_t* count_out;   /* (1) */
+  int64_t* slots;       /* extend: (T) */
+  int64_t table_stride;
+} fa_kv_table_params;
+int fa_kv_extend(const fa_kv_table_params* p, void* stream);
+int fa_kv_release(const fa_kv_table_params* p, void* stream);
+
+/*
  * Reads the device-side status word of `device` into out[0..7] (synchronises the
  * device).  out[0] != 0 means a kernel abandoned a bounded wait; out[1..5] hold
  * kernel id, block x, block y, wait site and loop iteration.  Returns FA_OK or

@@ -4,7 +4,8 @@ Public interface (same names and signatures as the reference project):
     flash_attention_fn, flash_attention_qkvpacked_fn,
     FlashAttentionFn, FlashAttentionQKVPackedFn
 plus, with no counterpart in the reference: FlashAttention (nn.Module), flash_attention_op
-(the same call through torch.library operators) and shard_batch_heads.
+(the same call through torch.library operators), shard_batch_heads, and for serving a paged key / value
+cache: PagedKVCache, paged_attention_fn, paged_kv_extend, paged_kv_write, paged_kv_release.
 """
 from .flash_attention import (  # noqa: F401
     FlashAttentionFn,
@@ -13,6 +14,13 @@ from .flash_attention import (  # noqa: F401
     flash_attention_qkvpacked_fn,
 )
 from .module import FlashAttention, flash_attention_op  # noqa: F401
+from .paged import (  # noqa: F401
+    PagedKVCache,
+    paged_attention_fn,
+    paged_kv_extend,
+    paged_kv_release,
+    paged_kv_write,
+)
 from .sharding import shard_batch_heads  # noqa: F401
 
 __all__ = [
@@ -23,4 +31,9 @@ __all__ = [
     "FlashAttention",
     "flash_attention_op",
     "shard_batch_heads",
+    "PagedKVCache",
+    "paged_attention_fn",
+    "paged_kv_extend",
+    "paged_kv_release",
+    "paged_kv_write",
 ]

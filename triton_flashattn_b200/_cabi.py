@@ -16,6 +16,7 @@ FA_F16, FA_BF16 = 0, 1
 FA_BIAS_NONE, FA_BIAS_SAME, FA_BIAS_BOOL, FA_BIAS_F32 = 0, 1, 2, 3
 FA_OK = 0
 
+_I64x2 = ctypes.c_int64 * 2
 _I64x3 = ctypes.c_int64 * 3
 
 
@@ -62,6 +63,49 @@ class FaParams(ctypes.Structure):
     ]
 
 
+def _fields(*groups):
+    """(name, type) pairs of `(type, "name name ...")` groups."""
+    return [(name, t) for t, names in groups for name in names.split()]
+
+
+class FaPagedParams(ctypes.Structure):
+    """Mirror of `struct fa_paged_params`."""
+
+    _fields_ = _fields(
+        (ctypes.c_uint32, "struct_size"),
+        (ctypes.c_int32, "device B H Hkv D page_size width num_pages dtype bias_kind"),
+        (ctypes.c_float, "sm_scale"),
+        (ctypes.c_void_p, "q k_cache v_cache o block_table seq_lens bias"),
+        (_I64x2, "q_stride o_stride"),
+        (_I64x3, "k_stride v_stride"),
+        (_I64x2, "bias_stride"),
+        (ctypes.c_int64, "table_stride"),
+    )
+
+
+class FaKvWriteParams(ctypes.Structure):
+    """Mirror of `struct fa_kv_write_params`."""
+
+    _fields_ = _fields(
+        (ctypes.c_uint32, "struct_size"),
+        (ctypes.c_int32, "device T Hkv D page_size num_pages reserved"),
+        (ctypes.c_void_p, "k v k_cache v_cache slots"),
+        (_I64x2, "k_stride v_stride"),
+        (_I64x3, "k_cache_stride v_cache_stride"),
+    )
+
+
+class FaKvTableParams(ctypes.Structure):
+    """Mirror of `struct fa_kv_table_params`."""
+
+    _fields_ = _fields(
+        (ctypes.c_uint32, "struct_size"),
+        (ctypes.c_int32, "device B width page_size capacity T reserved"),
+        (ctypes.c_void_p, "block_table lens change finished free_pages count lens_out count_out slots"),
+        (ctypes.c_int64, "table_stride"),
+    )
+
+
 EXPORTED_SYMBOLS = (
     "fa_version",
     "fa_launch_count",
@@ -80,6 +124,11 @@ EXPORTED_SYMBOLS = (
     "fa_bwd_pre",
     "fa_bwd_dkdv",
     "fa_bwd_dq",
+    "fa_paged_fwd",
+    "fa_paged_workspace_bytes",
+    "fa_kv_write",
+    "fa_kv_extend",
+    "fa_kv_release",
     "fa_last_device_status",
     "fa_reset_device_status",
     "fa_set_status_mirror",
@@ -119,6 +168,14 @@ def load() -> ctypes.CDLL:
     lib.fa_bwd_workspace_bytes.argtypes = [P]
     lib.fa_bwd_workspace.restype = ctypes.c_int
     lib.fa_bwd_workspace.argtypes = [P, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
+    lib.fa_paged_workspace_bytes.restype = ctypes.c_uint64
+    lib.fa_paged_workspace_bytes.argtypes = [ctypes.POINTER(FaPagedParams)]
+    lib.fa_paged_fwd.restype = ctypes.c_int
+    lib.fa_paged_fwd.argtypes = [ctypes.POINTER(FaPagedParams), ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
+    for name, params in (("fa_kv_write", FaKvWriteParams), ("fa_kv_extend", FaKvTableParams), ("fa_kv_release", FaKvTableParams)):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
     lib.fa_last_device_status.restype = ctypes.c_int
     lib.fa_last_device_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int32)]
     lib.fa_reset_device_status.restype = ctypes.c_int

@@ -289,6 +289,66 @@ int bwd_whole(const fa_params& p, cudaStream_t s, int* st) {
   return launch_bwd_dq(p, s, st);
 }
 
+// Base address and strides (in 16-bit elements) that 16-byte accesses need.
+template <int N>
+bool aligned16(const void* ptr, const int64_t (&s)[N]) {
+  bool ok = reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
+  for (int64_t x : s) ok = ok && x % 8 == 0;
+  return ok;
+}
+bool head_dim_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
+
+int validate_paged(const fa_paged_params* p) {
+  if (!p) return FA_ERR_NULL;
+  if (p->struct_size != sizeof(fa_paged_params)) return FA_ERR_ABI;
+  if (p->B < 1 || p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0 || !head_dim_ok(p->D)) return FA_ERR_SHAPE;
+  if (p->page_size < 1 || p->width < 1 || p->num_pages < 1) return FA_ERR_SHAPE;
+  if (p->dtype != FA_F16 && p->dtype != FA_BF16) return FA_ERR_DTYPE;
+  if (p->bias_kind < FA_BIAS_NONE || p->bias_kind > FA_BIAS_F32) return FA_ERR_DTYPE;
+  if (!p->q || !p->k_cache || !p->v_cache || !p->o || !p->block_table || !p->seq_lens) return FA_ERR_NULL;
+  if (p->bias_kind != FA_BIAS_NONE && !p->bias) return FA_ERR_NULL;
+  // positions, and the rows of all sequences, are counted in 32 bits
+  if (static_cast<int64_t>(p->width) * p->page_size > INT32_MAX - 4096 || static_cast<int64_t>(p->B) * p->H > INT32_MAX / 2)
+    return FA_ERR_TOO_LARGE;
+  if (!aligned16(p->q, p->q_stride) || !aligned16(p->o, p->o_stride) || !aligned16(p->k_cache, p->k_stride) ||
+      !aligned16(p->v_cache, p->v_stride))
+    return FA_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(p->block_table) % 4 || reinterpret_cast<uintptr_t>(p->seq_lens) % 4) return FA_ERR_ALIGN;
+  if (p->bias_kind != FA_BIAS_NONE && !element_aligned(p->bias, p->bias_kind)) return FA_ERR_ALIGN;
+  return FA_OK;
+}
+
+int validate_kv_write(const fa_kv_write_params* p) {
+  if (!p) return FA_ERR_NULL;
+  if (p->struct_size != sizeof(fa_kv_write_params)) return FA_ERR_ABI;
+  if (p->T < 0 || p->Hkv < 1 || !head_dim_ok(p->D) || p->page_size < 1 || p->num_pages < 1) return FA_ERR_SHAPE;
+  if (p->T == 0) return FA_OK;
+  if (!p->k || !p->v || !p->k_cache || !p->v_cache || !p->slots) return FA_ERR_NULL;
+  if (!aligned16(p->k, p->k_stride) || !aligned16(p->v, p->v_stride) || !aligned16(p->k_cache, p->k_cache_stride) ||
+      !aligned16(p->v_cache, p->v_cache_stride) || reinterpret_cast<uintptr_t>(p->slots) % 8)
+    return FA_ERR_ALIGN;
+  const int extent[3] = {p->num_pages, p->page_size, p->Hkv};
+  for (int i = 0; i < 3; ++i)  // every element has a place of its own
+    if (extent[i] > 1 && (p->k_cache_stride[i] <= 0 || p->v_cache_stride[i] <= 0)) return FA_ERR_ALIGN;
+  return FA_OK;
+}
+
+int validate_kv_table(const fa_kv_table_params* p, bool extend) {
+  if (!p) return FA_ERR_NULL;
+  if (p->struct_size != sizeof(fa_kv_table_params)) return FA_ERR_ABI;
+  if (p->B < 0 || p->width < 1 || p->page_size < 1 || p->capacity < 0 || (extend && p->T < 0)) return FA_ERR_SHAPE;
+  if (!p->count || !p->count_out || (p->capacity > 0 && !p->free_pages) || (extend && p->T > 0 && !p->slots)) return FA_ERR_NULL;
+  if (p->B > 0 && (!p->block_table || !p->lens || !p->lens_out || !(extend ? static_cast<const void*>(p->change) : p->finished)))
+    return FA_ERR_NULL;
+  if (static_cast<int64_t>(p->width) * p->page_size > INT32_MAX) return FA_ERR_TOO_LARGE;
+  if (p->B > 1 && p->table_stride < p->width) return FA_ERR_SHAPE;  // rows that share entries
+  const void* words[] = {p->block_table, p->lens, extend ? p->change : nullptr, p->free_pages, p->count, p->lens_out, p->count_out};
+  for (const void* w : words)
+    if (reinterpret_cast<uintptr_t>(w) % 4) return FA_ERR_ALIGN;
+  if (extend && reinterpret_cast<uintptr_t>(p->slots) % 8) return FA_ERR_ALIGN;
+  return FA_OK;
+}
+
 // The row copies count the bytes of a row, and places up to 16 bytes behind its end, in 32 bits.
 bool row_fits_copy(int N, int elem_bytes) { return static_cast<int64_t>(N) * elem_bytes <= INT32_MAX - 16; }
 
@@ -380,6 +440,45 @@ int fa_pack_rows(void* dst, const void* src, int64_t pitch, int elem_bytes, int6
   return with_device(device, [&](int*) {
     return launch_pack_rows(dst, src, pitch, elem_bytes, rows, N, static_cast<cudaStream_t>(stream));
   });
+}
+
+uint64_t fa_paged_workspace_bytes(const fa_paged_params* p) {
+  if (validate_paged(p)) return 0;
+  uint64_t bytes = 0;
+  with_device(p->device, [&](int*) {
+    bytes = paged_workspace_bytes(*p);
+    return (int)FA_OK;
+  });
+  return bytes;
+}
+
+int fa_paged_fwd(const fa_paged_params* p, void* workspace, uint64_t bytes, void* stream) {
+  int r = validate_paged(p);
+  if (r) return r;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return FA_ERR_ALIGN;
+  return with_device(p->device, [&](int* st) {
+    const uint64_t need = paged_workspace_bytes(*p);
+    if (need > 0 && (!workspace || bytes < need)) return (int)FA_ERR_NULL;
+    return launch_paged(*p, workspace, static_cast<cudaStream_t>(stream), st);
+  });
+}
+
+int fa_kv_write(const fa_kv_write_params* p, void* stream) {
+  int r = validate_kv_write(p);
+  if (r || p->T == 0) return r;
+  return with_device(p->device, [&](int* st) { return launch_kv_write(*p, static_cast<cudaStream_t>(stream), st); });
+}
+
+int fa_kv_extend(const fa_kv_table_params* p, void* stream) {
+  int r = validate_kv_table(p, true);
+  if (r) return r;
+  return with_device(p->device, [&](int* st) { return launch_kv_extend(*p, static_cast<cudaStream_t>(stream), st); });
+}
+
+int fa_kv_release(const fa_kv_table_params* p, void* stream) {
+  int r = validate_kv_table(p, false);
+  if (r) return r;
+  return with_device(p->device, [&](int* st) { return launch_kv_release(*p, static_cast<cudaStream_t>(stream), st); });
 }
 
 int fa_bwd_pre(const fa_params* p, void* stream) {

@@ -49,6 +49,12 @@ int check_tiled_bias(const fa_params& p, bool bwd);
 int launch_pad_rows(void* dst, const int64_t dst_stride[3], const void* src, const int64_t src_stride[3], int eb, int B, int H, int M,
                     int N, cudaStream_t stream);
 int launch_pack_rows(void* dst, const void* src, int64_t pitch, int eb, int64_t rows, int N, cudaStream_t stream);
+// Paged cache: attention of one new token a sequence (fa_paged.cu), rows into the pages and the tables (fa_kv.cu).
+uint64_t paged_workspace_bytes(const fa_paged_params& p);
+int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream, int* status);
+int launch_kv_write(const fa_kv_write_params& p, cudaStream_t stream, int* status);
+int launch_kv_extend(const fa_kv_table_params& p, cudaStream_t stream, int* status);
+int launch_kv_release(const fa_kv_table_params& p, cudaStream_t stream, int* status);
 int launch_bwd_pre(const fa_params& p, cudaStream_t stream, int* status);
 // How a causal dK/dV launch of head dims up to 128 over `n_bh` problems walks its tiles (see plan_dkdv), and how long its
 // longest CTA works then, in quarters of a step; 0 where that was not looked at (pairs, many tiles a CTA).

@@ -508,6 +508,277 @@ Tensor attention(const Tensor& a, const Tensor& k, const Tensor& v, const Tensor
   return out;
 }
 
+// ---------------------------------------------------------------------------- paged cache
+// Refuses what would lose a gradient or a transform: these operators serve, they have no derivative.
+void no_derivative(const char* what, std::initializer_list<const Tensor*> inputs) {
+  if (const auto& transforms = at::functorch::functorchTLSAccessor()) transforms->checkSupportsCppAutogradFunction();
+  for (const Tensor* t : inputs) {
+    if (!t->defined()) continue;
+    if (t->_fw_grad(0).defined()) fail(PyExc_NotImplementedError, std::string(what) + " has no forward-mode derivative (jvp)");
+    if (at::GradMode::is_enabled() && t->requires_grad())
+      fail(PyExc_NotImplementedError, std::string(what) + " has no backward: call it under torch.no_grad()");
+  }
+}
+
+void want_shape(const Tensor& t, const char* name, at::IntArrayRef want, const char* letters) {
+  if (t.sizes() != want)
+    fail(PyExc_ValueError, std::string(name) + " must have shape " + letters + " = " + shape_text(want) + ", got " + shape_text(t.sizes()));
+}
+void want_int32(const Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kInt) fail(PyExc_TypeError, std::string(name) + " must be an int32 tensor, got " + toString(t.scalar_type()));
+}
+void want_device(const Tensor& t, const char* name, const Tensor& like) {
+  if (!t.is_cuda() || t.device() != like.device())
+    fail(PyExc_ValueError, std::string(name) + " must live on the CUDA device of the other arguments (there is no CPU path)");
+}
+void want_int32_range(int64_t x, const char* what) {
+  if (x > INT32_MAX) fail(PyExc_ValueError, std::string(what) + " is too large");
+}
+
+// A pair of caches as the kernels take it; it is never copied.
+struct Cache {
+  int64_t pages, page_size, Hkv, D;
+};
+Cache check_caches(const Tensor& k, const Tensor& v) {
+  if (k.dim() != 4 || v.dim() != 4) fail(PyExc_ValueError, "k_cache, v_cache must be 4-D: (pages, page_size, Hkv, D)");
+  if (v.sizes() != k.sizes()) fail(PyExc_ValueError, "v_cache must have the shape of k_cache");
+  const Cache c{k.size(0), k.size(1), k.size(2), k.size(3)};
+  check_head_dim(c.D);
+  if (c.pages < 1 || c.page_size < 1 || c.Hkv < 1) fail(PyExc_ValueError, "a cache has at least one page, one token a page and one head");
+  want_int32_range(c.pages, "the number of pages");
+  want_int32_range(c.page_size, "the page size");
+  want_int32_range(c.Hkv, "the number of heads");
+  for (const Tensor* t : {&k, &v}) {
+    const auto st = t->strides();
+    if (st[3] != 1 || (st[0] | st[1] | st[2]) % 8 != 0 || reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 != 0)
+      fail(PyExc_ValueError, "k_cache, v_cache need a unit inner stride, and strides and an address that are multiples of 16 bytes");
+  }
+  return c;
+}
+// (B, H, D) or (T, Hkv, D) rows with 16-byte aligned strides; copied only when needed.
+Tensor rows_ready(const Tensor& t) {
+  const auto st = t.strides();
+  if (st[2] == 1 && (st[0] | st[1]) % 8 == 0 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+// What autograd compares to notice that a saved tensor was written to.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const Tensor& bias,
+                       PyObject* scale_obj) {
+  no_derivative("paged attention", {&q, &kc, &vc, &bias});
+  if (q.dim() != 3) fail(PyExc_ValueError, "q must be 3-D: (B, H, D), one new token a sequence");
+  const Cache c = check_caches(kc, vc);
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
+  if (D != c.D) fail(PyExc_AssertionError, "q and the caches must share the head dimension");
+  if (H < 1 || H % c.Hkv != 0) fail(PyExc_ValueError, "the heads of q must be a multiple of those of the caches");
+  check_dtype(q.scalar_type(), kc.scalar_type(), vc.scalar_type());
+  want_int32(table, "block_table");
+  want_int32(lens, "seq_lens");
+  if (table.dim() != 2 || table.size(0) != B || table.size(1) < 1)
+    fail(PyExc_ValueError, "block_table must be (B, pages of a sequence) with B = " + std::to_string(B) + ", got " + shape_text(table.sizes()));
+  want_shape(lens, "seq_lens", {B}, "(B,)");
+  if (!q.is_cuda() || kc.device() != q.device() || vc.device() != q.device())
+    fail(PyExc_ValueError, "q, k_cache, v_cache must live on the same CUDA device (there is no CPU path)");
+  want_device(table, "block_table", q);
+  want_device(lens, "seq_lens", q);
+  want_int32_range(B, "the number of sequences");
+  want_int32_range(H, "the number of heads");
+  want_int32_range(table.size(1), "the width of block_table");
+  if (bias.defined()) {
+    want_shape(bias, "bias", {B, H, table.size(1) * c.page_size}, "(B, H, width of block_table * page_size)");
+    want_device(bias, "bias", q);
+    if (bias.scalar_type() != at::kBool && !at::isFloatingType(bias.scalar_type()))
+      fail(PyExc_TypeError, std::string("bias must be a bool or floating tensor, got ") + toString(bias.scalar_type()));
+  }
+  const double scale = scale_of(scale_obj, D);
+  const int device = q.get_device();
+  require_health_words(device);
+
+  pybind11::gil_scoped_release no_gil;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  at::AutoDispatchBelowADInplaceOrView below;
+  raise_if_unhealthy(device);
+  Tensor out = empty_on(q, {B, H, D}, q.scalar_type());
+  if (B == 0) return out;
+  const Tensor tq = rows_ready(q), tl = dense(lens), tt = table.stride(1) == 1 ? table : table.contiguous();
+  Tensor tb;
+  fa_paged_params p{};
+  p.bias_kind = FA_BIAS_NONE;
+  if (bias.defined()) {
+    const auto dt = bias.scalar_type();
+    p.bias_kind = dt == at::kBool ? FA_BIAS_BOOL : dt == q.scalar_type() ? FA_BIAS_SAME : FA_BIAS_F32;
+    tb = p.bias_kind == FA_BIAS_F32 && dt != at::kFloat ? bias.to(at::kFloat) : bias;
+    if (tb.stride(2) != 1) tb = tb.contiguous();
+    p.bias = tb.const_data_ptr();
+    p.bias_stride[0] = tb.stride(0), p.bias_stride[1] = tb.stride(1);
+  }
+  p.struct_size = sizeof(fa_paged_params);
+  p.device = device;
+  p.B = static_cast<int32_t>(B), p.H = static_cast<int32_t>(H), p.Hkv = static_cast<int32_t>(c.Hkv), p.D = static_cast<int32_t>(D);
+  p.page_size = static_cast<int32_t>(c.page_size), p.width = static_cast<int32_t>(table.size(1));
+  p.num_pages = static_cast<int32_t>(c.pages);
+  p.dtype = q.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_F16;
+  p.sm_scale = static_cast<float>(scale);
+  p.q = tq.const_data_ptr(), p.k_cache = kc.const_data_ptr(), p.v_cache = vc.const_data_ptr(), p.o = out.mutable_data_ptr();
+  p.block_table = tt.const_data_ptr<int32_t>(), p.seq_lens = tl.const_data_ptr<int32_t>();
+  for (int i = 0; i < 2; ++i) p.q_stride[i] = tq.stride(i), p.o_stride[i] = out.stride(i);
+  for (int i = 0; i < 3; ++i) p.k_stride[i] = kc.stride(i), p.v_stride[i] = vc.stride(i);
+  p.table_stride = tt.stride(0);
+  const uint64_t bytes = fa_paged_workspace_bytes(&p);
+  Tensor ws;
+  if (bytes > 0) ws = empty_on(q, {static_cast<int64_t>(bytes)}, at::kByte);
+  check_code(fa_paged_fwd(&p, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(device)), "fa_paged_fwd");
+  return out;
+}
+
+void paged_kv_write(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& slots) {
+  no_derivative("paged_kv_write", {&k, &v, &kc, &vc});
+  const Cache c = check_caches(kc, vc);
+  if (k.dim() != 3 || v.dim() != 3) fail(PyExc_ValueError, "k, v must be 3-D: (T, Hkv, D)");
+  const int64_t T = k.size(0);
+  want_shape(k, "k", {T, c.Hkv, c.D}, "(T, Hkv, D)");
+  want_shape(v, "v", {T, c.Hkv, c.D}, "(T, Hkv, D)");
+  want_shape(slots, "slot_mapping", {T}, "(T,)");
+  check_dtype(k.scalar_type(), v.scalar_type(), k.scalar_type());
+  if (kc.scalar_type() != k.scalar_type() || vc.scalar_type() != k.scalar_type())
+    fail(PyExc_TypeError, "k, v and the caches must share one dtype");
+  if (slots.scalar_type() != at::kLong) fail(PyExc_TypeError, std::string("slot_mapping must be an int64 tensor, got ") + toString(slots.scalar_type()));
+  for (const Tensor* t : {&kc, &vc})
+    for (int i = 0; i < 3; ++i)
+      if (t->size(i) > 1 && t->stride(i) <= 0) fail(PyExc_ValueError, "the caches must not be expanded views: they are written to");
+  if (!k.is_cuda() || v.device() != k.device() || kc.device() != k.device() || vc.device() != k.device() || slots.device() != k.device())
+    fail(PyExc_ValueError, "k, v, k_cache, v_cache, slot_mapping must live on the same CUDA device (there is no CPU path)");
+  want_int32_range(T, "the number of tokens");
+  const int device = k.get_device();
+  require_health_words(device);
+
+  pybind11::gil_scoped_release no_gil;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  at::AutoDispatchBelowADInplaceOrView below;
+  raise_if_unhealthy(device);
+  if (T == 0) return;
+  const Tensor tk = rows_ready(k), tv = rows_ready(v), ts = dense(slots);
+  fa_kv_write_params p{};
+  p.struct_size = sizeof(fa_kv_write_params);
+  p.device = device;
+  p.T = static_cast<int32_t>(T), p.Hkv = static_cast<int32_t>(c.Hkv), p.D = static_cast<int32_t>(c.D);
+  p.page_size = static_cast<int32_t>(c.page_size), p.num_pages = static_cast<int32_t>(c.pages);
+  p.k = tk.const_data_ptr(), p.v = tv.const_data_ptr();
+  p.k_cache = kc.mutable_data_ptr(), p.v_cache = vc.mutable_data_ptr();
+  p.slots = ts.const_data_ptr<int64_t>();
+  for (int i = 0; i < 2; ++i) p.k_stride[i] = tk.stride(i), p.v_stride[i] = tv.stride(i);
+  for (int i = 0; i < 3; ++i) p.k_cache_stride[i] = kc.stride(i), p.v_cache_stride[i] = vc.stride(i);
+  check_code(fa_kv_write(&p, stream_of(device)), "fa_kv_write");
+  written(kc);
+  written(vc);
+}
+
+// What extend and release share: checks, the places of the results (the inputs' own when `inplace`), the parameters.
+struct Tables {
+  fa_kv_table_params p{};
+  Tensor lens, count, lens_out, count_out;  // kept alive over the call
+};
+void check_tables(const Tensor& table, const Tensor& lens, const Tensor& stack, const Tensor& count, int64_t page_size) {
+  want_int32(table, "block_table");
+  want_int32(lens, "seq_lens");
+  want_int32(stack, "free_pages");
+  want_int32(count, "free_count");
+  if (table.dim() != 2 || table.size(1) < 1) fail(PyExc_ValueError, "block_table must be (B, pages of a sequence), got " + shape_text(table.sizes()));
+  want_shape(lens, "seq_lens", {table.size(0)}, "(B,)");
+  if (stack.dim() != 1 || !stack.is_contiguous()) fail(PyExc_ValueError, "free_pages must be a dense 1-D tensor");
+  if (count.numel() != 1) fail(PyExc_ValueError, "free_count must hold one number");
+  if (page_size < 1) fail(PyExc_ValueError, "page_size must be at least 1");
+  want_int32_range(table.size(0), "the number of requests");
+  want_int32_range(table.size(1), "the width of block_table");
+  want_int32_range(stack.numel(), "the number of pages");
+  want_int32_range(page_size, "the page size");
+  if (table.size(1) * page_size > INT32_MAX) fail(PyExc_ValueError, "a row of block_table holds more tokens than 32 bits count");
+  if (!table.is_cuda()) fail(PyExc_ValueError, "block_table must live on a CUDA device (there is no CPU path)");
+  want_device(lens, "seq_lens", table);
+  want_device(stack, "free_pages", table);
+  want_device(count, "free_count", table);
+}
+Tables make_tables(const Tensor& table, const Tensor& lens, const Tensor& stack, const Tensor& count, int64_t page_size, bool inplace) {
+  Tables t;
+  t.lens = dense(lens);
+  t.count = count;
+  t.lens_out = inplace ? lens : empty_on(table, lens.sizes(), at::kInt);
+  t.count_out = inplace ? count : empty_on(table, count.sizes(), at::kInt);
+  fa_kv_table_params& p = t.p;
+  p.struct_size = sizeof(fa_kv_table_params);
+  p.device = table.get_device();
+  p.B = static_cast<int32_t>(table.size(0)), p.width = static_cast<int32_t>(table.size(1));
+  p.page_size = static_cast<int32_t>(page_size), p.capacity = static_cast<int32_t>(stack.numel());
+  p.block_table = table.mutable_data_ptr<int32_t>();
+  p.table_stride = table.stride(0);
+  p.lens = t.lens.const_data_ptr<int32_t>();
+  p.free_pages = stack.mutable_data_ptr<int32_t>();
+  p.count = count.const_data_ptr<int32_t>();
+  p.lens_out = t.lens_out.mutable_data_ptr<int32_t>();
+  p.count_out = t.count_out.mutable_data_ptr<int32_t>();
+  return t;
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_kv_extend(const Tensor& table, const Tensor& lens, const Tensor& more, const Tensor& stack,
+                                                   const Tensor& count, int64_t page_size, int64_t num_tokens, bool inplace) {
+  no_derivative("paged_kv_extend", {});
+  check_tables(table, lens, stack, count, page_size);
+  if (table.stride(1) != 1 || (table.size(0) > 1 && table.stride(0) < table.size(1)))
+    fail(PyExc_ValueError, "block_table needs rows of their own with a unit inner stride: it is written to");
+  want_int32(more, "new_lens");
+  want_shape(more, "new_lens", {table.size(0)}, "(B,)");
+  want_device(more, "new_lens", table);
+  if (inplace && !lens.is_contiguous()) fail(PyExc_ValueError, "seq_lens must be dense when it is written to");
+  if (num_tokens < 0) fail(PyExc_ValueError, "num_tokens must not be negative");
+  want_int32_range(num_tokens, "the number of tokens");
+  const int device = table.get_device();
+  require_health_words(device);
+
+  pybind11::gil_scoped_release no_gil;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  at::AutoDispatchBelowADInplaceOrView below;
+  raise_if_unhealthy(device);
+  Tables t = make_tables(table, lens, stack, count, page_size, inplace);
+  const Tensor tm = dense(more);
+  Tensor slots = empty_on(table, {num_tokens}, at::kLong);
+  t.p.change = tm.const_data_ptr<int32_t>();
+  t.p.slots = slots.mutable_data_ptr<int64_t>();
+  t.p.T = static_cast<int32_t>(num_tokens);
+  check_code(fa_kv_extend(&t.p, stream_of(device)), "fa_kv_extend");
+  written(table);
+  if (inplace) written(lens), written(count);
+  return {std::move(slots), std::move(t.lens_out), std::move(t.count_out)};
+}
+
+std::tuple<Tensor, Tensor> paged_kv_release(const Tensor& table, const Tensor& lens, const Tensor& finished, const Tensor& stack,
+                                            const Tensor& count, int64_t page_size, bool inplace) {
+  no_derivative("paged_kv_release", {});
+  check_tables(table, lens, stack, count, page_size);
+  if (finished.scalar_type() != at::kBool) fail(PyExc_TypeError, std::string("finished must be a bool tensor, got ") + toString(finished.scalar_type()));
+  want_shape(finished, "finished", {table.size(0)}, "(B,)");
+  want_device(finished, "finished", table);
+  if (inplace && !lens.is_contiguous()) fail(PyExc_ValueError, "seq_lens must be dense when it is written to");
+  const int device = table.get_device();
+  require_health_words(device);
+
+  pybind11::gil_scoped_release no_gil;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  at::AutoDispatchBelowADInplaceOrView below;
+  raise_if_unhealthy(device);
+  const Tensor rows = table.stride(1) == 1 && (table.size(0) <= 1 || table.stride(0) >= table.size(1)) ? table : table.contiguous();
+  Tables t = make_tables(rows, lens, stack, count, page_size, inplace);
+  const Tensor tf = dense(finished);
+  t.p.finished = reinterpret_cast<const uint8_t*>(tf.const_data_ptr<bool>());
+  check_code(fa_kv_release(&t.p, stream_of(device)), "fa_kv_release");
+  written(stack);
+  if (inplace) written(lens), written(count);
+  return {std::move(t.lens_out), std::move(t.count_out)};
+}
+
 // ---------------------------------------------------------------------------- Python entry points
 Tensor tensor_arg(PyObject* o, const char* name, bool optional = false) {
   if (optional && o == Py_None) return Tensor();
@@ -617,6 +888,61 @@ PyObject* py_classify_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+int64_t int_arg(PyObject* o, const char* name) {
+  THPObjectPtr number(PyNumber_Index(o));
+  if (!number) {
+    PyErr_Clear();
+    fail(PyExc_TypeError, std::string(name) + " must be a whole number, got " + Py_TYPE(o)->tp_name);
+  }
+  const long long x = PyLong_AsLongLong(number.get());
+  if (x == -1 && PyErr_Occurred()) throw python_error();
+  return x;
+}
+
+// paged_attention(q, k_cache, v_cache, block_table, seq_lens, bias | None, sm_scale | None) -> out
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 7, "paged_attention");
+    return THPVariable_Wrap(paged_attention(tensor_arg(a[0], "q"), tensor_arg(a[1], "k_cache"), tensor_arg(a[2], "v_cache"),
+                                            tensor_arg(a[3], "block_table"), tensor_arg(a[4], "seq_lens"),
+                                            tensor_arg(a[5], "bias", true), a[6]));
+  });
+}
+
+// paged_kv_write(k, v, k_cache, v_cache, slot_mapping): fills the slots
+PyObject* py_paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 5, "paged_kv_write");
+    paged_kv_write(tensor_arg(a[0], "k"), tensor_arg(a[1], "v"), tensor_arg(a[2], "k_cache"), tensor_arg(a[3], "v_cache"),
+                   tensor_arg(a[4], "slot_mapping"));
+    Py_RETURN_NONE;
+  });
+}
+
+// paged_kv_extend(block_table, seq_lens, new_lens, free_pages, free_count, page_size, num_tokens, inplace) -> (slots, lens, count)
+PyObject* py_paged_kv_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 8, "paged_kv_extend");
+    auto [slots, lens, count] =
+        paged_kv_extend(tensor_arg(a[0], "block_table"), tensor_arg(a[1], "seq_lens"), tensor_arg(a[2], "new_lens"),
+                        tensor_arg(a[3], "free_pages"), tensor_arg(a[4], "free_count"), int_arg(a[5], "page_size"),
+                        int_arg(a[6], "num_tokens"), truth(a[7]));
+    return PyTuple_Pack(3, THPObjectPtr(THPVariable_Wrap(slots)).get(), THPObjectPtr(THPVariable_Wrap(lens)).get(),
+                        THPObjectPtr(THPVariable_Wrap(count)).get());
+  });
+}
+
+// paged_kv_release(block_table, seq_lens, finished, free_pages, free_count, page_size, inplace) -> (lens, count)
+PyObject* py_paged_kv_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 7, "paged_kv_release");
+    auto [lens, count] =
+        paged_kv_release(tensor_arg(a[0], "block_table"), tensor_arg(a[1], "seq_lens"), tensor_arg(a[2], "finished"),
+                         tensor_arg(a[3], "free_pages"), tensor_arg(a[4], "free_count"), int_arg(a[5], "page_size"), truth(a[6]));
+    return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(lens)).get(), THPObjectPtr(THPVariable_Wrap(count)).get());
+  });
+}
+
 // set_health_registrar(callable(device) -> address of the int32[8] host words)
 PyObject* py_set_health_registrar(PyObject*, PyObject* cb) {
   Py_INCREF(cb);
@@ -631,6 +957,10 @@ PyMethodDef kMethods[] = {
     {"fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_fwd)), METH_FASTCALL, nullptr},
     {"bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_bwd)), METH_FASTCALL, nullptr},
     {"classify_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_classify_bias)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_paged_attention)), METH_FASTCALL, nullptr},
+    {"paged_kv_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_paged_kv_write)), METH_FASTCALL, nullptr},
+    {"paged_kv_extend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_paged_kv_extend)), METH_FASTCALL, nullptr},
+    {"paged_kv_release", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_paged_kv_release)), METH_FASTCALL, nullptr},
     {"set_health_registrar", py_set_health_registrar, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
