@@ -31,6 +31,10 @@ SOURCES = [
     "fa_decode.cu",
     "fa_small.cu",
     "fa_paged.cu",
+    "fa_paged_bf16.cu",
+    "fa_paged_bf16_rows.cu",
+    "fa_paged_f16.cu",
+    "fa_paged_f16_rows.cu",
     "fa_kv.cu",
     "fa_copy.cu",
     "fa_bwd_pre.cu",

@@ -307,8 +307,8 @@ int validate_paged(const fa_paged_params* p) {
   if (p->bias_kind < FA_BIAS_NONE || p->bias_kind > FA_BIAS_F32) return FA_ERR_DTYPE;
   if (!p->q || !p->k_cache || !p->v_cache || !p->o || !p->block_table || !p->seq_lens) return FA_ERR_NULL;
   if (p->bias_kind != FA_BIAS_NONE && !p->bias) return FA_ERR_NULL;
-  // positions, and the rows of all sequences, are counted in 32 bits
-  if (static_cast<int64_t>(p->width) * p->page_size > INT32_MAX - 4096 || static_cast<int64_t>(p->B) * p->H > INT32_MAX / 2)
+  // positions, and the heads of all sequences, are counted in 32 bits
+  if (static_cast<int64_t>(p->width) * p->page_size > INT32_MAX - 4096 || static_cast<int64_t>(p->B) * p->H > 1 << 24)
     return FA_ERR_TOO_LARGE;
   if (!aligned16(p->q, p->q_stride) || !aligned16(p->o, p->o_stride) || !aligned16(p->k_cache, p->k_stride) ||
       !aligned16(p->v_cache, p->v_stride))

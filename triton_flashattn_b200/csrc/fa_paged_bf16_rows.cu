@@ -1,0 +1,6 @@
+// The paged attention kernels for bf16, a copy for each row.
+#include "fa_paged.cuh"
+
+namespace fa {
+template int launch_paged_kernels<__nv_bfloat16, false>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
+}  // namespace fa
