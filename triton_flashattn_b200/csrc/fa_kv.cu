@@ -10,7 +10,21 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// Division, rounded down, of x < 2^31 by 1 <= d < 2^31: with 2^(s - 1) < d <= 2^s it is (x + x * mul / 2^32) >> s,
+// mul = 2^32 (2^s - d) / d + 1.
+struct Divisor {
+  uint32_t mul, shift;
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (__umulhi(x, mul) + x) >> shift; }
+};
+Divisor divisor(uint64_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {static_cast<uint32_t>((((1ull << s) - d) << 32) / d + 1), s};
+}
+
 // ---- rows into the pages -----------------------------------------------------------------------
+// A copy: what bounds it is the memory, read once, written once.  A thread moves 16 bytes of K and of V of kAhead tokens; all its
+// loads are under way before the first store.
 struct WriteParams {
   const uint16_t* k;
   const uint16_t* v;
@@ -21,32 +35,54 @@ struct WriteParams {
   int64_t k_sT, k_sH, v_sT, v_sH;
   int64_t kc_sP, kc_sT, kc_sH, vc_sP, vc_sT, vc_sH;
   int64_t n_slots, chunks;  // slots of the cache; 16-byte pieces of a tensor of rows
-  int page_size, Hkv, per_head;
+  Divisor row, page;        // pieces of a token; tokens of a page
+  int page_size, row_chunks, head_shift;  // 2^head_shift pieces of a head
 };
 
-__global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
+constexpr int kWriteThreads = 256;
+constexpr int kAhead = 4;
+
+template <typename I>
+__global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WriteParams p) {
   grid_dep_launch_next();
+  const I first = static_cast<I>(blockIdx.x) * (kWriteThreads * kAhead) + threadIdx.x;
+  uint32_t token[kAhead], head[kAhead], d[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const I i = first + j * kWriteThreads;
+    token[j] = sizeof(I) == 4 ? p.row.of(static_cast<uint32_t>(i)) : static_cast<uint32_t>(i / p.row_chunks);
+    const uint32_t c = static_cast<uint32_t>(i - static_cast<I>(token[j]) * p.row_chunks);
+    head[j] = c >> p.head_shift;
+    d[j] = (c - (head[j] << p.head_shift)) * 8;
+  }
   grid_dep_wait();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= p.chunks || *reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const int64_t row = i / p.per_head;
-  const int d = static_cast<int>(i - row * p.per_head) * 8;
-  const int64_t t = row / p.Hkv;
-  const int h = static_cast<int>(row - t * p.Hkv);
-  const int64_t slot = __ldcg(p.slots + t);
-  if (slot < 0 || slot >= p.n_slots) return;
-  const int64_t page = slot / p.page_size;
-  const int at = static_cast<int>(slot - page * p.page_size);
-  const uint4 k = __ldcg(reinterpret_cast<const uint4*>(p.k + t * p.k_sT + h * p.k_sH + d));
-  const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p.v + t * p.v_sT + h * p.v_sH + d));
-  *reinterpret_cast<uint4*>(p.k_cache + page * p.kc_sP + at * p.kc_sT + h * p.kc_sH + d) = k;
-  *reinterpret_cast<uint4*>(p.v_cache + page * p.vc_sP + at * p.vc_sT + h * p.vc_sH + d) = v;
+  const int status = *reinterpret_cast<volatile int*>(p.status);
+  int64_t slot[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) slot[j] = first + j * kWriteThreads < static_cast<I>(p.chunks) ? __ldcg(p.slots + token[j]) : -1;
+  if (status != 0) return;
+  uint4 k[kAhead], v[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    if (slot[j] < 0 || slot[j] >= p.n_slots) continue;
+    k[j] = __ldcg(reinterpret_cast<const uint4*>(p.k + token[j] * p.k_sT + head[j] * p.k_sH + d[j]));
+    v[j] = __ldcg(reinterpret_cast<const uint4*>(p.v + token[j] * p.v_sT + head[j] * p.v_sH + d[j]));
+  }
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    if (slot[j] < 0 || slot[j] >= p.n_slots) continue;
+    const int64_t page = slot[j] >> 31 ? slot[j] / p.page_size : p.page.of(static_cast<uint32_t>(slot[j]));
+    const int64_t at = slot[j] - page * p.page_size;
+    *reinterpret_cast<uint4*>(p.k_cache + page * p.kc_sP + at * p.kc_sT + head[j] * p.kc_sH + d[j]) = k[j];
+    *reinterpret_cast<uint4*>(p.v_cache + page * p.vc_sP + at * p.vc_sT + head[j] * p.vc_sH + d[j]) = v[j];
+  }
 }
 
 // ---- tables ------------------------------------------------------------------------------------
-// One cluster of CTAs does a call.  All of them look at all requests, kThreads at a time, and have the same running sums; what
-// is written (pages, slots) is shared out over their threads.  The cluster barrier between looking and writing lets lens_out be
-// lens and count_out be count.
+// All CTAs of a call look at all requests, kThreads at a time, and have the same running sums; what is written (pages, slots) is
+// shared out over their warps, a run of neighbours each, so that a lane looks for the request of its first one, and again only
+// where its next one is another's.  Where lens_out is lens or count_out is count, the CTAs are one cluster, with a barrier between looking and writing.
+// What bounds a call is latency: a launch, the lengths, the pages, the stores.
 constexpr int kThreads = 512;
 
 struct TableParams {
@@ -62,6 +98,8 @@ struct TableParams {
   int* status;
   int64_t table_stride;
   int B, width, page_size, capacity, T;
+  int in_place;
+  Divisor page;
 };
 
 // Running sum of x over the threads of a CTA, x itself not included; *total is the sum of all.
@@ -98,95 +136,138 @@ __device__ __forceinline__ int find(const int64_t* first, int n, int64_t x) {
   return lo;
 }
 
-__device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_size) { return (tokens + page_size - 1) / page_size; }
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, const TableParams& p) {
+  const int64_t x = tokens + p.page_size - 1;
+  return x >> 31 ? x / p.page_size : p.page.of(static_cast<uint32_t>(x));
+}
+
+__device__ __forceinline__ void all_here(const TableParams& p) {
+  if (p.in_place && gridDim.x > 1) cg::this_cluster().sync();
+  else __syncthreads();
+}
+
+// What is between `from` and `to` (a list whose owners' first entries are in first[0 .. n - 1]) is dealt out to the warps of the
+// call in runs, a lane an entry: into(owner, entry, *at(owner, entry)), where at() may be null (-1 then).  Four loads of a lane
+// are under way at a time.
+template <typename At, typename Into>
+__device__ __forceinline__ void for_each(int64_t from, int64_t to, const int64_t* first, int n, At at, Into into) {
+  constexpr int kAtOnce = 4;
+  const int lane = threadIdx.x & 31;
+  const int warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), warps = gridDim.x * (kThreads / 32);
+  const int64_t run = ((to - from + warps - 1) / warps + 31) / 32 * 32;
+  const int64_t begin = from + warp * run, end = min(begin + run, to);
+  if (begin >= end) return;
+  int owner = find(first, n, min(begin + lane, end - 1));
+  int64_t next = owner + 1 < n ? first[owner + 1] : to;
+  for (int64_t x0 = begin + lane; x0 < end; x0 += 32 * kAtOnce) {
+    int owners[kAtOnce], value[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t x = x0 + 32 * j;
+      if (x >= next && x < end) {
+        owner += find(first + owner, n - owner, x);
+        next = owner + 1 < n ? first[owner + 1] : to;
+      }
+      owners[j] = owner;
+      const int* src = x < end ? at(owner, x) : nullptr;
+      value[j] = src ? __ldcg(src) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (x0 + 32 * j < end) into(owners[j], x0 + 32 * j, value[j]);
+  }
+}
 
 __global__ void __launch_bounds__(kThreads) kv_extend_kernel(const TableParams p) {
   __shared__ int64_t sums[kThreads / 32];
   __shared__ int64_t s_off[kThreads], s_rank[kThreads];  // tokens, pages wanted before each request
-  __shared__ int s_old[kThreads];
+  __shared__ int s_old[kThreads], s_have[kThreads];
   __shared__ uint8_t s_granted[kThreads];
-  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ int s_taken;
   const int tid = threadIdx.x;
-  const int me = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
   grid_dep_launch_next();
+  if (tid == 0) s_taken = 0;
   grid_dep_wait();
-  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;  // (the same for all CTAs)
+  const int status = *reinterpret_cast<volatile int*>(p.status);
   const int64_t count = min(max(__ldcg(p.count), 0), p.capacity);
-  int64_t tokens = 0, wanted = 0, taken = 0;  // of the requests looked at so far
+  int64_t tokens = 0, wanted = 0;  // of the requests looked at so far
+  int taken = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + tid, n = min(kThreads, p.B - b0);
-    const int raw = b < p.B ? __ldcg(p.lens + b) : 0;
-    const int64_t old = max(raw, 0), more = b < p.B ? max(__ldcg(p.change + b), 0) : 0;
-    int64_t chunk_tokens, chunk_wanted, chunk_taken;
+    const int raw = b < p.B ? __ldcg(p.lens + b) : 0, change = b < p.B ? __ldcg(p.change + b) : 0;
+    if (status != 0) return;  // (the same for all CTAs)
+    const int64_t old = max(raw, 0), more = max(change, 0);
+    int64_t chunk_tokens, chunk_wanted;
     const int64_t off = tokens + scan(more, sums, &chunk_tokens);
     const bool fits = old + more <= static_cast<int64_t>(p.width) * p.page_size && off + more <= p.T;
-    const int64_t need = fits ? pages_of(old + more, p.page_size) - pages_of(old, p.page_size) : 0;
+    const int64_t have = pages_of(old, p), need = fits ? pages_of(old + more, p) - have : 0;
     const int64_t rank = wanted + scan(need, sums, &chunk_wanted);
     const bool granted = fits && (need == 0 || rank + need <= count);
-    scan(granted ? need : 0, sums, &chunk_taken);
     s_off[tid] = off;
     s_rank[tid] = rank;
     s_old[tid] = static_cast<int>(old);
+    s_have[tid] = static_cast<int>(have);
     s_granted[tid] = granted;
-    cluster.sync();  // all have looked at these requests
-    if (blockIdx.x == 0 && b < p.B) p.lens_out[b] = granted ? static_cast<int>(old + more) : raw;
     // granted requests take a run of pages from `wanted` on: behind the first that got none nobody gets any
-    for (int64_t x = wanted + me; x < wanted + chunk_taken; x += all) {
-      const int i = find(s_rank, n, x);
-      const int64_t at = pages_of(s_old[i], p.page_size) + x - s_rank[i];
-      p.table[(b0 + i) * p.table_stride + at] = __ldcg(p.free_pages + (count - 1 - x));
-    }
-    const int64_t end = min(tokens + chunk_tokens, static_cast<int64_t>(p.T));
-    for (int64_t t = tokens + me; t < end; t += all) {
-      const int i = find(s_off, n, t);
-      int64_t slot = -1;
-      if (s_granted[i]) {
-        const int64_t pos = s_old[i] + t - s_off[i], at = pos / p.page_size, have = pages_of(s_old[i], p.page_size);
-        const int page = at < have ? __ldcg(p.table + (b0 + i) * p.table_stride + at)
-                                   : __ldcg(p.free_pages + (count - 1 - (s_rank[i] + at - have)));
-        if (page >= 0) slot = static_cast<int64_t>(page) * p.page_size + pos % p.page_size;
-      }
-      p.slots[t] = slot;
-    }
+    const int most = __reduce_max_sync(0xffffffffu, granted && need > 0 ? static_cast<int>(rank + need) : 0);
+    if ((tid & 31) == 0 && most > 0) atomicMax(&s_taken, most);
+    all_here(p);  // all have looked at these requests
+    if (blockIdx.x == 0 && b < p.B) p.lens_out[b] = granted ? static_cast<int>(old + more) : raw;
+    const int taken_now = s_taken;
+    for_each(
+        min(wanted, static_cast<int64_t>(taken_now)), taken_now, s_rank, n, [&](int, int64_t x) { return p.free_pages + (count - 1 - x); },
+        [&](int i, int64_t x, int page) { p.table[(b0 + i) * p.table_stride + s_have[i] + (x - s_rank[i])] = page; });
+    for_each(
+        tokens, min(tokens + chunk_tokens, static_cast<int64_t>(p.T)), s_off, n,
+        [&](int i, int64_t x) -> const int* {
+          if (!s_granted[i]) return nullptr;
+          const int at = static_cast<int>(p.page.of(static_cast<uint32_t>(s_old[i] + (x - s_off[i])))), have = s_have[i];
+          return at < have ? p.table + (b0 + i) * p.table_stride + at : p.free_pages + (count - 1 - (s_rank[i] + at - have));
+        },
+        [&](int i, int64_t x, int page) {
+          const uint32_t pos = static_cast<uint32_t>(s_old[i] + (x - s_off[i]));
+          p.slots[x] = page < 0 ? -1 : static_cast<int64_t>(page) * p.page_size + (pos - p.page.of(pos) * p.page_size);
+        });
     tokens += chunk_tokens;
     wanted += chunk_wanted;
-    taken += chunk_taken;
+    taken = taken_now;
     __syncthreads();  // the next requests' sums go over these
   }
+  if (status != 0) return;
+  const int64_t me = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
   for (int64_t t = min(tokens, static_cast<int64_t>(p.T)) + me; t < p.T; t += all) p.slots[t] = -1;
-  cluster.sync();  // all have read the count
-  if (me == 0) *p.count_out = static_cast<int>(count - taken);
+  all_here(p);  // all have read the count
+  if (me == 0) *p.count_out = static_cast<int>(count) - taken;
 }
 
 __global__ void __launch_bounds__(kThreads) kv_release_kernel(const TableParams p) {
   __shared__ int64_t sums[kThreads / 32];
   __shared__ int64_t s_rank[kThreads];
-  cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x;
-  const int me = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
   grid_dep_launch_next();
   grid_dep_wait();
-  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int status = *reinterpret_cast<volatile int*>(p.status);
   int64_t top = min(max(__ldcg(p.count), 0), p.capacity);
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + tid, n = min(kThreads, p.B - b0);
     const int raw = b < p.B ? __ldcg(p.lens + b) : 0;
     const bool gone = b < p.B && __ldcg(p.finished + b) != 0;
-    const int64_t give = gone ? min(pages_of(max(raw, 0), p.page_size), static_cast<int64_t>(p.width)) : 0;
+    if (status != 0) return;
+    const int64_t give = gone ? min(pages_of(max(raw, 0), p), static_cast<int64_t>(p.width)) : 0;
     int64_t chunk;
     s_rank[tid] = scan(give, sums, &chunk);
-    cluster.sync();
+    all_here(p);
     if (blockIdx.x == 0 && b < p.B) p.lens_out[b] = gone ? 0 : raw;
-    const int64_t end = min(chunk, p.capacity - top);
-    for (int64_t x = me; x < end; x += all) {
-      const int i = find(s_rank, n, x);
-      p.free_pages[top + x] = __ldcg(p.table + (b0 + i) * p.table_stride + (x - s_rank[i]));
-    }
+    for_each(
+        0, min(chunk, p.capacity - top), s_rank, n,
+        [&](int i, int64_t x) { return p.table + (b0 + i) * p.table_stride + (x - s_rank[i]); },
+        [&](int, int64_t x, int page) { p.free_pages[top + x] = page; });
     top = min(top + chunk, static_cast<int64_t>(p.capacity));
     __syncthreads();
   }
-  cluster.sync();
-  if (me == 0) *p.count_out = static_cast<int>(top);
+  if (status != 0) return;
+  all_here(p);
+  if (blockIdx.x == 0 && tid == 0) *p.count_out = static_cast<int>(top);
 }
 
 TableParams table_params(const fa_kv_table_params& p, int* status) {
@@ -203,6 +284,8 @@ TableParams table_params(const fa_kv_table_params& p, int* status) {
   t.status = status;
   t.table_stride = p.table_stride;
   t.B = p.B, t.width = p.width, t.page_size = p.page_size, t.capacity = p.capacity, t.T = p.T;
+  t.page = divisor(p.page_size);
+  t.in_place = p.lens_out == p.lens || p.count_out == p.count;
   return t;
 }
 
@@ -220,21 +303,38 @@ int launch_kv_write(const fa_kv_write_params& p, cudaStream_t stream, int* statu
   w.kc_sP = p.k_cache_stride[0], w.kc_sT = p.k_cache_stride[1], w.kc_sH = p.k_cache_stride[2];
   w.vc_sP = p.v_cache_stride[0], w.vc_sT = p.v_cache_stride[1], w.vc_sH = p.v_cache_stride[2];
   w.n_slots = static_cast<int64_t>(p.num_pages) * p.page_size;
-  w.page_size = p.page_size, w.Hkv = p.Hkv, w.per_head = p.D / 8;
-  w.chunks = static_cast<int64_t>(p.T) * p.Hkv * w.per_head;
-  const int64_t blocks = (w.chunks + 255) / 256;
+  w.page_size = p.page_size;
+  for (w.head_shift = 1; 8 << w.head_shift < p.D;) ++w.head_shift;
+  const int64_t row_chunks = static_cast<int64_t>(p.Hkv) << w.head_shift;
+  if (row_chunks > INT32_MAX) return FA_ERR_TOO_LARGE;
+  w.row_chunks = static_cast<int>(row_chunks);
+  w.row = divisor(row_chunks), w.page = divisor(p.page_size);
+  w.chunks = p.T * row_chunks;
+  constexpr int kPerBlock = kWriteThreads * kAhead;
+  const int64_t blocks = (w.chunks + kPerBlock - 1) / kPerBlock;
   if (blocks > INT32_MAX) return FA_ERR_TOO_LARGE;
-  return launch_overlapped(kv_write_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, w);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  return blocks * kPerBlock <= INT32_MAX ? launch_overlapped(kv_write_kernel<uint32_t>, grid, kWriteThreads, 0, stream, w)
+                                         : launch_overlapped(kv_write_kernel<uint64_t>, grid, kWriteThreads, 0, stream, w);
+}
+
+// CTAs for so many entries: a run of 64 for each warp, as far as a cluster goes where one is needed.
+static int table_ctas(int64_t entries, bool in_place) {
+  const int64_t ctas = (entries + 64 * (kThreads / 32) - 1) / (64 * (kThreads / 32)), most = in_place ? 8 : 64;
+  return static_cast<int>(ctas < 1 ? 1 : ctas < most ? ctas : most);
 }
 
 int launch_kv_extend(const fa_kv_table_params& p, cudaStream_t stream, int* status) {
-  const int ctas = p.T <= 4 * kThreads ? 1 : 8;
-  return launch_overlapped(kv_extend_kernel, dim3(ctas), kThreads, 0, stream, table_params(p, status), ctas);
+  const TableParams t = table_params(p, status);
+  const int ctas = table_ctas(p.T, t.in_place);
+  return launch_overlapped(kv_extend_kernel, dim3(ctas), kThreads, 0, stream, t, t.in_place ? ctas : 1);
 }
 
 int launch_kv_release(const fa_kv_table_params& p, cudaStream_t stream, int* status) {
-  const int ctas = static_cast<int64_t>(p.B) * p.width <= 4 * kThreads ? 1 : 8;
-  return launch_overlapped(kv_release_kernel, dim3(ctas), kThreads, 0, stream, table_params(p, status), ctas);
+  const TableParams t = table_params(p, status);
+  const int64_t pages = static_cast<int64_t>(p.B) * p.width;
+  const int ctas = table_ctas(pages < p.capacity ? pages : p.capacity, t.in_place);
+  return launch_overlapped(kv_release_kernel, dim3(ctas), kThreads, 0, stream, t, t.in_place ? ctas : 1);
 }
 
 }  // namespace fa
