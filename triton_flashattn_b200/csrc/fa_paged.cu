@@ -8,14 +8,7 @@ namespace {
 // Sequences of at most this many keys are not split over CTAs: one launch less.
 constexpr int kWholeKeys = 64;
 
-// Bytes of a ring place and of the queries, as Cfg has them.
-struct Room {
-  int tile, queries;
-};
-Room room_of(int DP, int NQ, bool tiles) {
-  return {(DP == 64 ? 2 : 1) * 16 * (tiles ? 2 * DP : 2 * DP + 16), 8 * NQ * DP * 2};
-}
-PagedPlan plan_paged(const fa_paged_params& p, bool tiles) {
+PagedPlan plan_paged(const fa_paged_params& p) {
   PagedPlan x;
   const int heads = p.H / p.Hkv;
   x.DP = padded_head_dim(p.D);
@@ -23,10 +16,10 @@ PagedPlan plan_paged(const fa_paged_params& p, bool tiles) {
   x.splits = (heads + 8 * x.NQ - 1) / (8 * x.NQ);
   x.rows = (heads + x.splits - 1) / x.splits;
   x.units = p.Hkv * x.splits;
-  const Room room = room_of(x.DP, x.NQ, tiles);
+  const int tile = (x.DP == 64 ? 2 : 1) * 32 * x.DP, queries = 8 * x.NQ * x.DP * 2;  // bytes, as Cfg has them
   // Warps: as many as there is room for, fewer where that spares parts (each has units / gcd items over 1 / parts of the
   // stretch: a warp a unit, or some units, or some warps a unit).
-  const auto ring_of = [&](int warps) { return ((kPagedSmem / warps) / 1024 * 1024 - room.queries) / (2 * room.tile); };
+  const auto ring_of = [&](int warps) { return ((kPagedSmem / warps) / 1024 * 1024 - queries) / (2 * tile); };
   int most = kMostWarps;
   while (most > 4 && ring_of(most) < 2) --most;
   x.warps = 0;
@@ -47,7 +40,7 @@ PagedPlan plan_paged(const fa_paged_params& p, bool tiles) {
   x.whole = cap <= kWholeKeys;
   if (x.whole) x.parts = 1;
   const int stretches = x.ctas * x.parts;
-  x.by_seq = p.B <= stretches;
+  x.by_seq = p.B <= kFew || p.B <= stretches;
   x.joints = x.by_seq ? p.B : stretches;
   // More teams while a team has several rounds of sums and the SMs room for them; of smaller slices where a block holds no more.
   x.ahead = x.by_seq ? 8 : 4;  // (elsewhere a sequence has two sums, rarely more)
@@ -82,29 +75,22 @@ bool cache_map(CUtensorMap* out, const void* base, const fa_paged_params& p, con
   const uint32_t box[4] = {64, 1, 16, 1};
   return make_tmap_4d(out, base, 2, dims, strides, box) == FA_OK;
 }
-bool tiled_pages(const fa_paged_params& p) { return p.page_size % 16 == 0; }
 
 }  // namespace
 
-// (with what the larger of the two kinds of copies takes: whether the cache has a tile map is known at the launch)
 uint64_t paged_workspace_bytes(const fa_paged_params& p) {
-  uint64_t most = 0;
-  for (int tiles = 0; tiles <= (tiled_pages(p) ? 1 : 0); ++tiles) {
-    const PagedPlan x = plan_paged(p, tiles != 0);
-    const uint64_t bytes = x.whole ? 0 : part_bytes(x) + 16ull * x.joints;
-    most = bytes > most ? bytes : most;
-  }
-  return most;
+  const PagedPlan x = plan_paged(p);
+  return x.whole ? 0 : part_bytes(x) + 16ull * x.joints;
 }
 
 int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream, int* status) {
   PagedParams d;
-  const bool aligned = tiled_pages(p) && cache_map(&d.k_map, p.k_cache, p, p.k_stride) && cache_map(&d.v_map, p.v_cache, p, p.v_stride);
-  const PagedPlan x = plan_paged(p, aligned);
+  const bool aligned = p.page_size % 16 == 0 && cache_map(&d.k_map, p.k_cache, p, p.k_stride) && cache_map(&d.v_map, p.v_cache, p, p.v_stride);
+  const PagedPlan x = plan_paged(p);
   d.q = p.q, d.k = p.k_cache, d.v = p.v_cache, d.bias = p.bias, d.o = p.o;
   d.table = p.block_table, d.lens = p.seq_lens, d.status = status;
   d.part = static_cast<float*>(workspace);
-  d.joint = workspace ? reinterpret_cast<int4*>(static_cast<char*>(workspace) + part_bytes(x)) : nullptr;
+  d.joint = x.whole || p.B <= kFew ? nullptr : reinterpret_cast<int4*>(static_cast<char*>(workspace) + part_bytes(x));
   d.q_sB = p.q_stride[0], d.q_sH = p.q_stride[1], d.o_sB = p.o_stride[0], d.o_sH = p.o_stride[1];
   d.k_sP = p.k_stride[0], d.k_sT = p.k_stride[1], d.k_sH = p.k_stride[2];
   d.v_sP = p.v_stride[0], d.v_sT = p.v_stride[1], d.v_sH = p.v_stride[2];
@@ -112,7 +98,7 @@ int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream,
   d.B = p.B, d.H = p.H, d.Hkv = p.Hkv, d.D = p.D;
   d.page_size = p.page_size, d.num_pages = p.num_pages, d.width = p.width, d.page_tiles = p.page_size / 16;
   d.heads = p.H / p.Hkv, d.rows = x.rows, d.splits = x.splits, d.units = x.units;
-  d.parts = x.parts, d.ring = x.ring, d.whole = x.whole ? 1 : 0, d.by_seq = x.by_seq ? 1 : 0, d.joints = x.joints, d.slices = x.slices, d.teams = x.teams;
+  d.parts = x.parts, d.ring = x.ring, d.whole = x.whole ? 1 : 0, d.by_seq = x.by_seq ? 1 : 0, d.joints = x.joints, d.ctas = x.ctas, d.slices = x.slices, d.teams = x.teams;
   d.scale = p.bias_kind == FA_BIAS_NONE || p.bias_kind == FA_BIAS_BOOL ? p.sm_scale * kLog2e : p.sm_scale;
   // Division by d, rounded down, of x < 2^31: with 2^(s - 1) < d <= 2^s it is (x + x * mul / 2^32) >> s, mul = 2^32 (2^s - d) / d + 1.
   const auto divisor = [](uint64_t by, uint32_t& mul, uint32_t& shift) {
@@ -123,11 +109,8 @@ int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream,
   };
   divisor(aligned ? p.page_size / 16 : p.page_size, d.div_mul, d.div_shift);
   divisor(x.splits, d.splits_mul, d.splits_shift);
-  if (p.dtype == FA_BF16)
-    return aligned ? launch_paged_kernels<__nv_bfloat16, true>(d, x, p.bias_kind, stream)
-                   : launch_paged_kernels<__nv_bfloat16, false>(d, x, p.bias_kind, stream);
-  return aligned ? launch_paged_kernels<__half, true>(d, x, p.bias_kind, stream)
-                 : launch_paged_kernels<__half, false>(d, x, p.bias_kind, stream);
+  if (p.dtype == FA_BF16) return (aligned ? launch_paged_bf16_tiles : launch_paged_bf16_rows)(d, x, p.bias_kind, stream);
+  return (aligned ? launch_paged_f16_tiles : launch_paged_f16_rows)(d, x, p.bias_kind, stream);
 }
 
 }  // namespace fa

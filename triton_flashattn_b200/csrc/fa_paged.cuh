@@ -34,7 +34,8 @@ struct PagedParams {
   const int* lens;
   int* status;
   float* part;  // workspace: unfinished sums [stretch][2][unit][row]: of the sequence that began before, of the one that goes on
-  int4* joint;  // workspace: a sequence that goes on: it (-1: none), the first and the last stretch that have some of it
+  int4* joint;  // workspace: a sequence that goes on: it (-1: none), the first and the last stretch that have some of it.  Null for
+                // few sequences, where the joining kernel finds out itself, and where none goes on
   int64_t q_sB, q_sH, o_sB, o_sH, k_sP, k_sT, k_sH, v_sP, v_sT, v_sH, bias_sB, bias_sH, table_s;
   int B, H, Hkv, D;
   int page_size, num_pages, width, page_tiles;
@@ -47,14 +48,39 @@ struct PagedParams {
   int parts;   // stretches of a CTA
   int ring;    // tiles that a warp has room for
   int whole;   // stretches are whole sequences
+  int ctas;    // of the first kernel
   int by_seq;  // joint has an entry for each sequence (else for each stretch)
   int joints;  // entries of it
   int slices, teams;  // of a (sequence, head) in the joining kernel
   float scale;  // of the scores; in log2 units unless there is a float bias
 };
 
-constexpr int kKernelId = 20;  // in the status word
+// How a call is cut: rows a unit, units a key head, warps, their ring, the grid.
+struct PagedPlan {
+  int DP, NQ, rows, splits, units;
+  int warps, ring, parts;
+  int ctas, joints, slices, teams, ahead;
+  bool whole, by_seq;
+};
+constexpr int kPagedSmem = 218 * 1024;  // shared memory for the warps' rooms
+
+// An unfinished sum: per row DP values, their maximum and the sum of the weights (and two words to keep rows at 16 bytes).
+__host__ __device__ constexpr int row_floats(int DP) { return DP + 4; }
+
+// The kernels of a type and a kind of copies, each pair in a translation unit of its own.
+int launch_paged_bf16_tiles(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+int launch_paged_bf16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+int launch_paged_f16_tiles(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+int launch_paged_f16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+
 constexpr int kMostWarps = 8;
+// Up to this many sequences a lane has one, and the places of the sequences are known without tables.
+constexpr int kFew = 32;
+constexpr int kJoinThreads = 256;
+
+namespace {
+
+constexpr int kKernelId = 20;  // in the status word
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&a)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -74,14 +100,12 @@ __device__ __forceinline__ void tma_load_4d_to(uint32_t dst, const CUtensorMap* 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-// A row of `bytes` (a multiple of 16, both addresses too); its arrival counts on the barrier.
-__device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// An arrival on the barrier once all copies that this thread has asked for so far have landed.
+__device__ __forceinline__ void arrive_when_landed(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -137,57 +161,89 @@ __device__ __forceinline__ float weight_of(float m, float m_all) {
 // What the sums are multiplied with in the end: 0 without a key; and where the sum is NaN, as those it belongs to then are.
 __device__ __forceinline__ float inverse(float m, float sum) { return m != -INFINITY && sum > 0.f ? 1.f / sum : 0.f; }
 
+// An element of a bias or mask as it lies in memory, and what it stands for.  (Loaded into whole registers: nothing waits for it
+// before it is used.)
+template <int BIAS>
+constexpr int kBiasBytes = BIAS == 2 ? 1 : BIAS == 3 ? 4 : 2;
+template <int BIAS>
+__device__ __forceinline__ uint32_t load_bias(const void* p) {
+  uint32_t x;
+  if constexpr (BIAS == 2) asm volatile("ld.global.u8 %0, [%1];" : "=r"(x) : "l"(p));
+  else if constexpr (BIAS == 3) asm volatile("ld.global.u32 %0, [%1];" : "=r"(x) : "l"(p));
+  else asm volatile("ld.global.u16 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
+}
 template <int BIAS, typename T>
-struct BiasType {
-  using type = float;
-};
-template <typename T>
-struct BiasType<1, T> {
-  using type = T;
-};
-template <typename T>
-struct BiasType<2, T> {
-  using type = uint8_t;
-};
+__device__ __forceinline__ float bias_of(uint32_t x) {
+  return BIAS == 3 ? __uint_as_float(x) : Pack2<T>::unpack(x).x;
+}
 
-// Shared memory of a kernel.  DP: head dim rounded up to 64, 128, 256; NQ: groups of 8 rows; TILES: tile copies.
-template <int DP, int NQ, bool TILES>
+// Shared memory of a kernel.  DP: head dim rounded up to 64, 128, 256; NQ: groups of 8 rows.
+template <int DP, int NQ>
 struct Cfg {
   static constexpr int kPieces = DP == 64 ? 2 : 1;  // of 16 keys, in a tile: what a warp waits for and works on at once
   static constexpr int kKeys = 16 * kPieces;
-  // bytes of 16 keys of K or V: rows of 128 bytes swizzled as the tile copies leave them, or whole rows and 16 bytes between
-  static constexpr int kPiece = 16 * (TILES ? 2 * DP : 2 * DP + 16);
+  static constexpr int kPiece = 32 * DP;  // bytes of 16 keys of K or V: blocks of 64 elements, rows of 128 bytes, swizzled
   static constexpr int kTile = kPieces * kPiece;
   static constexpr int kQ = 8 * NQ * DP * 2;            // the queries
-  static constexpr bool kQRegs = NQ == 1 && DP <= 128;  // which are kept in registers, and the next ones fetched meanwhile
+  static constexpr bool kQRegs = NQ == 1 && DP <= 128;  // are kept in registers over a sequence
   static constexpr int warp_bytes(int ring) { return (2 * ring * kTile + kQ + 1023) / 1024 * 1024; }
 };
-// An unfinished sum: per row DP values, their maximum and the sum of the weights (and two words to keep rows at 16 bytes).
-__host__ __device__ constexpr int row_floats(int DP) { return DP + 4; }
 
-// The line of tiles, and how the CTAs share it.
+// The line of tiles, and how the CTAs, and the parts of their stretches, share it.
 struct Line {
   int64_t tiles, share;
   int ctas, longer;  // the first `longer` CTAs take one tile more than `share`
+  __device__ __forceinline__ Line(int64_t tiles, int most) : tiles(tiles) {
+    ctas = static_cast<int>(min(static_cast<int64_t>(most), tiles));
+    share = divide(tiles, ctas);
+    longer = static_cast<int>(tiles - share * ctas);
+  }
   __device__ __forceinline__ int64_t begin(int cta) const { return cta * share + min(cta, longer); }
   __device__ __forceinline__ int cta_of(int64_t x) const {
     const int64_t turn = longer * (share + 1);
     return static_cast<int>(x < turn ? divide(x, share + 1) : longer + divide(x - turn, share));
   }
+  // The stretch that place x is in.
+  __device__ __forceinline__ int stretch_of(int64_t x, int parts) const {
+    const int cta = cta_of(x);
+    if (parts == 1) return cta;
+    const int64_t from = begin(cta);
+    return cta * parts + static_cast<int>(divide((x - from + 1) * parts - 1, begin(cta + 1) - from));
+  }
 };
+
+// The running sum over the lanes of a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t x) {
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
+    if (static_cast<int>(threadIdx.x & 31) >= off) x += y;
+  }
+  return x;
+}
+// Keys of sequence b, and their tiles.  (An empty sequence has a tile, as it has its zeros to write.)
+__device__ __forceinline__ int length_of(const PagedParams& p, int b) {
+  return min(max(__ldcg(p.lens + b), 0), p.width * p.page_size);
+}
+template <int KEYS>
+__device__ __forceinline__ int tiles_in(int len) {
+  return max((len + KEYS - 1) / KEYS, 1);
+}
 
 template <int DP, int NQ, typename T, int BIAS, bool TILES>
 __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_constant__ PagedParams p) {
   using P2 = Pack2<T>;
-  using C = Cfg<DP, NQ, TILES>;
-  using BT = typename BiasType<BIAS, T>::type;
+  using C = Cfg<DP, NQ>;
   constexpr int KS = DP / 16;  // steps of 16 head-dim elements
   constexpr int MB = C::kPieces, kMostRing = 8;
   constexpr int kMostThreads = kMostWarps * 32;
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[kMostWarps][kMostRing];  // K and V of a ring place have landed
-  __shared__ uint2 s_info[kMostWarps][kMostRing];  // of the tile there: its keys that exist; 1 the last of its sequence, 2 of the item
+  __shared__ __align__(8) uint64_t s_q_full[kMostWarps];           // the next queries have
+  // of the tile there: its keys that exist; 1 the last of its sequence, 2 of the item; the sequence's tiles
+  __shared__ __align__(16) uint4 s_info[kMostWarps][kMostRing];
   __shared__ int64_t s_before[kMostThreads + 1];   // tiles of the sequences before a thread's
   __shared__ int64_t s_sum[kMostWarps];
   __shared__ int s_abort;
@@ -195,16 +251,20 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, threads = blockDim.x;
   const int r = lane >> 2, t = lane & 3;
   const int cap = p.width * p.page_size, S = p.ring, units = p.units;
-  grid_dep_launch_next();
+  if (TILES && tid == 0) {
+    tma_prefetch_desc(&p.k_map);
+    tma_prefetch_desc(&p.v_map);
+  }
 
   // ---- this warp's room: a ring of tiles of K, one of V, queries
-  const int warp_bytes = (2 * S * C::kTile + C::kQ + 1023) / 1024 * 1024;
+  const int warp_bytes = C::warp_bytes(S);
   uint8_t* const room = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023) + warp * warp_bytes;
   const uint32_t ring = smem_u32(room), q_room = ring + 2 * S * C::kTile;
   uint64_t(&full)[kMostRing] = s_full[warp];
-  if (lane < S) mbar_init(&full[lane], 1);
+  if (lane < S) mbar_init(&full[lane], TILES ? 1 : 32);
+  if (lane == 0) mbar_init(&s_q_full[warp], 32);
   // What no copy writes is read all the same, times 0: columns behind the head dim, rows of queries that the unit has not, keys
-  // behind the last one.  (What an earlier tile left is as good as zeros; an infinite or NaN value would be put right, slowly.)
+  // behind the last one or on no page.  (What an earlier tile left is as good as zeros; an infinite or NaN value would be put right, slowly.)
   {
     const int from = TILES && MB == 1 ? 2 * S * C::kTile : 0;
     for (int i = from / 16 + lane; i < (2 * S * C::kTile + C::kQ) / 16; i += 32)
@@ -214,13 +274,18 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   mbar_fence_init();
   fence_proxy_async_smem();
 
+  // (For few sequences the joining kernel reads the lengths before this one has ended, so it may start once whatever wrote them
+  // has.)
+  const bool late = !p.whole && !p.joint;
+  if (!late) grid_dep_launch_next();
   grid_dep_wait();  // the previous kernel's results (and the status word) are visible from here
+  if (late) grid_dep_launch_next();
   const int status = *reinterpret_cast<volatile int*>(p.status);
-  const auto length = [&](int b) { return min(max(__ldcg(p.lens + b), 0), cap); };
-  const auto tiles_of = [&](int len) { return max((len + C::kKeys - 1) / C::kKeys, 1); };  // (an empty sequence has its zeros to write)
+  const auto length = [&](int b) { return length_of(p, b); };
+  const auto tiles_of = [&](int len) { return tiles_in<C::kKeys>(len); };
 
-  // ---- the line.  Up to 32 sequences: a lane has one.  More: a thread has some, and a table what lies before.
-  const bool few = p.B <= 32;
+  // ---- the line.  Few sequences: a lane has one.  More: a thread has some, and a table what lies before.
+  const bool few = p.B <= kFew;
   const int each = few ? 1 : (p.B + threads - 1) / threads;
   int64_t sum = 0;
   int len_l = 0;
@@ -228,36 +293,28 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     len_l = length(b);
     sum += tiles_of(len_l);
   }
-  int64_t upto = sum;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += x;
-  }
-  Line line;
+  const int64_t upto = warp_scan(sum);
+  int64_t tiles = 0;
   if (few) {
-    line.tiles = __shfl_sync(0xffffffffu, upto, 31);
+    tiles = __shfl_sync(0xffffffffu, upto, 31);
     __syncthreads();  // s_abort
   } else {
     if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
-    int64_t before = upto - sum, all = 0;
+    int64_t before = upto - sum;
     for (int w = 0; w < warps; ++w) {
       const int64_t x = s_sum[w];
       before += w < warp ? x : 0;
-      all += x;
+      tiles += x;
     }
     s_before[tid] = before;
-    line.tiles = all;
     __syncthreads();
   }
   if (status != 0) return;
-  line.ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), line.tiles));
-  line.share = divide(line.tiles, line.ctas);
-  line.longer = static_cast<int>(line.tiles - line.share * line.ctas);
+  const Line line(tiles, gridDim.x);
   const int me = blockIdx.x;
   if (me >= line.ctas) {
-    if (!p.whole && !p.by_seq && tid < p.parts) p.joint[me * p.parts + tid] = make_int4(-1, 0, 0, 0);
+    if (p.joint && !p.by_seq && tid < p.parts) p.joint[me * p.parts + tid] = make_int4(-1, 0, 0, 0);
     return;
   }
 
@@ -283,12 +340,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     int64_t before = s_before[lo];
     for (const int stop = min(b + each, p.B); b + 1 < stop;) {
       const int mine = b + lane < stop ? tiles_of(length(b + lane)) : 0;
-      int64_t sums = mine;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int64_t z = __shfl_up_sync(0xffffffffu, sums, off);
-        if (lane >= off) sums += z;
-      }
+      const int64_t sums = warp_scan(mine);
       const uint32_t beyond = __ballot_sync(0xffffffffu, before + sums > x);
       if (beyond) {
         const int k = __ffs(beyond) - 1;
@@ -376,7 +428,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
       if (!p.whole) {
         const int stretch = me * p.parts + x.part;
         if (lane < p.rows) *reinterpret_cast<float2*>(part_at(stretch, 0, x.unit) + lane * row_floats(DP) + DP) = make_float2(-INFINITY, 0.f);
-        if (lane == 0 && x.unit == 0 && !p.by_seq) p.joint[stretch] = make_int4(-1, 0, 0, 0);
+        if (lane == 0 && x.unit == 0 && p.joint && !p.by_seq) p.joint[stretch] = make_int4(-1, 0, 0, 0);
       }
     }
   };
@@ -385,7 +437,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   // The next tile: its key head, pages and first rows there (TILES: of each piece; else of the lane's key), its keys, and whether
   // it is the last one.
   int t_head = 0, t_page[TILES ? MB : 1], t_row[TILES ? MB : 1];
-  uint32_t t_keys = 0, t_last = 0;
+  uint32_t t_keys = 0, t_last = 0, t_tiles = 0;
   int t_rows = 0;      // with a bias: rows of its unit,
   int64_t t_bias = 0;  // and where theirs begins
   const auto turn_to_next = [&] {
@@ -410,6 +462,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
       t_row[0] = key - fast_div(key, p.div_mul, p.div_shift) * p.page_size;
       t_keys &= __ballot_sync(0xffffffffu, page_l >= 0);
     }
+    t_tiles = i_tiles;
     t_last = (i_tile + 1 == i_tiles ? 1u : 0u) | (i_left == 1 ? 2u : 0u);
     if constexpr (BIAS != 0) {
       const int m0 = (i_unit - i_head * p.splits) * p.rows;
@@ -433,7 +486,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     const uint32_t k_dst = ring + to * C::kTile, v_dst = ring + (S + to) * C::kTile;
     if constexpr (TILES) {
       if (elect_one()) {
-        s_info[warp][to] = make_uint2(t_keys, t_last);
+        s_info[warp][to] = make_uint4(t_keys, t_last, t_tiles, 0);
         // (a piece without a key is left out: what lies there, finite or not, counts for nothing)
         mbar_expect_tx(&full[to], MB == 2 && t_keys >> 16 ? 4 * C::kPiece : 2 * C::kPiece);
 #pragma unroll
@@ -447,17 +500,25 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           }
       }
     } else {
-      if (lane == 0) {
-        s_info[warp][to] = make_uint2(t_keys, t_last);
-        mbar_expect_tx(&full[to], 2 * __popc(t_keys) * p.D * 2);
+      // 16 bytes a lane; a lane knows the addresses of its own key, and asks for those of the row that it copies from
+      constexpr int kRow = DP / 8, kRows = 32 / kRow;  // pieces of a row, rows of a step
+      if (lane == 0) s_info[warp][to] = make_uint4(t_keys, t_last, t_tiles, 0);
+      const bool mine = t_keys >> lane & 1;
+      const T* k_src = static_cast<const T*>(p.k) + (mine ? t_page[0] * p.k_sP + t_row[0] * p.k_sT : 0) + t_head * p.k_sH;
+      const T* v_src = static_cast<const T*>(p.v) + (mine ? t_page[0] * p.v_sP + t_row[0] * p.v_sT : 0) + t_head * p.v_sH;
+      const int c = lane % kRow;
+#pragma unroll
+      for (int i = 0; i < C::kKeys / kRows; ++i) {
+        const int key = i * kRows + lane / kRow;
+        const T* ks = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k_src), key));
+        const T* vs = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v_src), key));
+        const uint32_t at = (key >> 4) * C::kPiece + (c >> 3) * 2048 + (key & 15) * 128 + (((c & 7) ^ (key & 7)) << 4);
+        if ((t_keys >> key & 1) && c * 8 < p.D) {
+          copy16_async(k_dst + at, ks + c * 8);
+          copy16_async(v_dst + at, vs + c * 8);
+        }
       }
-      __syncwarp();
-      if (t_keys >> lane & 1) {
-        copy_row(k_dst + lane * (2 * DP + 16), static_cast<const T*>(p.k) + t_page[0] * p.k_sP + t_row[0] * p.k_sT + t_head * p.k_sH,
-                 p.D * 2, &full[to]);
-        copy_row(v_dst + lane * (2 * DP + 16), static_cast<const T*>(p.v) + t_page[0] * p.v_sP + t_row[0] * p.v_sT + t_head * p.v_sH,
-                 p.D * 2, &full[to]);
-      }
+      arrive_when_landed(&full[to]);
     }
     __syncwarp();
   };
@@ -465,7 +526,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   const auto prefetch_bias = [&] {
     if constexpr (BIAS != 0) {
       if (lane < t_rows) {
-        const char* src = reinterpret_cast<const char*>(static_cast<const BT*>(p.bias) + t_bias + lane * p.bias_sH);
+        const char* src = static_cast<const char*>(p.bias) + (t_bias + lane * p.bias_sH) * kBiasBytes<BIAS>;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
       }
     }
@@ -480,6 +541,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
       const int m = i / (DP / 8), c = i % (DP / 8);
       if (m < rows && c * 8 < p.D) copy16_async(q_room + m * (2 * DP) + ((c ^ (m & 7)) << 4), src + m * p.q_sH + c * 8);
     }
+    arrive_when_landed(&s_q_full[warp]);
   };
 
   // the item and the place on the line that the products are at
@@ -497,13 +559,10 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   // ---- the products
   const uint32_t lane_row = (lane >> 3 & 1) * 8 + (lane & 7);  // K: rows 0-7 and 8-15 of 16 elements, then those of the next
   const uint32_t lane_key = (lane >> 4) * 8 + (lane & 7);      // V: 8 elements and the next of keys 0-7, then of keys 8-15
-  const uint32_t k_lane = TILES ? lane_row * 128 + (((lane >> 4) ^ (lane & 7)) << 4) : lane_row * (2 * DP + 16) + (lane >> 4) * 16;
-  const uint32_t v_lane =
-      TILES ? lane_key * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4) : lane_key * (2 * DP + 16) + (lane >> 3 & 1) * 16;
+  const uint32_t k_lane = lane_row * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = lane_key * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
   // elements 16 ks .. of the rows of a tile
-  const auto step_at = [&](uint32_t tile_lane, int ks) {
-    return TILES ? (tile_lane ^ ((2 * ks & 7) << 4)) + (ks >> 2) * 2048 : tile_lane + ks * 32;
-  };
+  const auto step_at = [&](uint32_t tile_lane, int ks) { return (tile_lane ^ ((2 * ks & 7) << 4)) + (ks >> 2) * 2048; };
   // elements 32 j .. of the queries of a group: B operands of two steps
   const auto q_step = [&](int g, int j) {
     return q_room + (g * 8 + (lane & 7)) * (2 * DP) + (((4 * j + (lane >> 3)) ^ (lane & 7)) << 4);
@@ -513,7 +572,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   uint32_t q[C::kQRegs ? KS / 2 : 1][4];
   float o[NQ][KS][4];         // O^T: [query group][16 head-dim rows][fragment]
   float mx[NQ][2], l[NQ][2];  // of rows 2t, 2t+1: running maximum, this lane's part of the sum
-  BT bf[NQ][MB][4];           // bias of the next tile, as it is
+  uint32_t bf[NQ][MB][4];     // bias of the next tile, as it lies in memory
   int h0 = 0, rows = 0;
   int64_t bias_bh = 0;
   const auto load_b = [&](int tile, uint32_t keys) {
@@ -526,18 +585,32 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           for (int i = 0; i < 4; ++i) {
             const int m = g * 8 + 2 * t + (i & 1), key = k * 16 + r + 8 * (i >> 1);
             if (m < rows && keys >> key & 1)
-              bf[g][k][i] = static_cast<const BT*>(p.bias)[bias_bh + m * p.bias_sH + tile * C::kKeys + key];
+              bf[g][k][i] =
+                  load_bias<BIAS>(static_cast<const char*>(p.bias) + (bias_bh + m * p.bias_sH + tile * C::kKeys + key) * kBiasBytes<BIAS>);
           }
     }
   };
 
+  // What follows the sequence that the products are at, once its last tile is there: the next of the item, or the next item.
+  int next_item = item, next_unit = unit, next_b = b + 1, next_tile = 0;
+  const auto open_next = [&] {
+    Item it;
+    for (next_item = item + warps; next_item < n_items; next_item += warps) {
+      it = item_at(next_item);
+      if (it.tiles > 0) break;
+    }
+    if (next_item >= n_items) return;
+    const Place at = start_of(it);
+    next_unit = it.unit, next_b = at.b, next_tile = at.tile;
+  };
+
   bool opens = true, begins = false;
   int place = 0;  // in the ring
-  uint32_t phase = 0;
+  uint32_t phase = 0, q_phase = 0;
   int x = 0;  // tiles done
 #pragma unroll 1
   while (true) {
-    const uint2 info = s_info[warp][place];
+    const uint4 info = s_info[warp][place];
     const uint32_t keys = info.x;
     const bool refill = i_item < n_items;
     if (refill) turn_to_next();
@@ -547,20 +620,11 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
       bias_bh = b * p.bias_sB + h0 * p.bias_sH;
       begins = tile == 0;
       load_b(tile, keys);
+      if (!wait_warp(&s_q_full[warp], q_phase, wait_ctx, 2, x)) break;
+      q_phase ^= 1;
       if constexpr (C::kQRegs) {
-        copies_landed();
-        __syncwarp();
 #pragma unroll
         for (int j = 0; j < KS / 2; ++j) ldsm_x4(q[j], q_step(0, j));
-        __syncwarp();
-        if (b + 1 < p.B) fetch_q(b + 1, unit);  // (of no use where the item ends before)
-      } else {
-        if (x > 0) {  // (the first ones are on their way)
-          __syncwarp();
-          fetch_q(b, unit);
-        }
-        copies_landed();
-        __syncwarp();
       }
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
@@ -611,6 +675,11 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[g][k][e] += s2[g][k][e];
     }
+    if (info.y != 0) {  // the last tile of this sequence or item: the next queries may come
+      __syncwarp();
+      if (info.y >> 1) open_next();
+      if (next_item < n_items) fetch_q(next_b, next_unit);
+    }
     // ---- scores, -inf where a key takes no part
     bool need = false;
 #pragma unroll
@@ -622,7 +691,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           float y = s[g][k][i] * p.scale;
           // a mask selects: whatever the score of a masked key is (infinite, NaN), it takes no part
           if constexpr (BIAS == 2) y = bf[g][k][i] ? y : -INFINITY;
-          else if constexpr (BIAS != 0) y += static_cast<float>(bf[g][k][i]);
+          else if constexpr (BIAS != 0) y += bias_of<BIAS, T>(bf[g][k][i]);
           if (!(keys >> (k * 16 + r + 8 * (i >> 1)) & 1)) y = -INFINITY;
           s[g][k][i] = y;
           need = need || y > mx[g][i & 1] + 8.f;
@@ -668,16 +737,20 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     // ---- O^T += V^T P^T
     // An infinite or NaN value: zero weights make it NaN.  So the values times zero are summed, and looked at.
     const uint32_t v_tile = ring + (S + place) * C::kTile + v_lane;
-    float odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float odd[4][4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd[c][e] = 0.f;
 #pragma unroll
     for (int k = 0; k < MB; ++k)
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         uint32_t a[4];
         ldsm_x4_trans(a, step_at(v_tile, i) + k * C::kPiece);
-        mma16816<T>(odd[i & 1], a, 0u, 0u);
+        mma16816<T>(odd[i & 3], a, 0u, 0u);
       }
-    if (__all_sync(0xffffffffu, odd[0][0] == 0.f && odd[0][2] == 0.f && odd[1][0] == 0.f && odd[1][2] == 0.f)) {
+    if (__all_sync(0xffffffffu, (odd[0][0] + odd[1][0]) + (odd[2][0] + odd[3][0]) + ((odd[0][2] + odd[1][2]) + (odd[2][2] + odd[3][2])) == 0.f)) {
 #pragma unroll
       for (int k = 0; k < MB; ++k)
 #pragma unroll
@@ -769,40 +842,21 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           if (r == 0) *reinterpret_cast<float2*>(dst + DP) = make_float2(mx[g][j], l[g][j]);
         }
     }
-    if (!p.whole && unit == 0 && lane == 0) {
+    if (p.joint && unit == 0 && lane == 0) {
       // the sequence that begins here: does it go on, and up to which stretch
       const int stretch = me * p.parts + item / units;
       if (begins && !ends) {
         const Item it = item_at(item);
-        const int64_t end = it.first + it.tiles - tile + tiles_of(length(b)) - 1;  // its last tile on the line
-        const int cta = line.cta_of(end);
-        const int64_t from = line.begin(cta), tiles = line.begin(cta + 1) - from;
-        const int part = static_cast<int>(divide((end - from + 1) * p.parts - 1, tiles));
-        p.joint[p.by_seq ? b : stretch] = make_int4(b, stretch, cta * p.parts + part, 0);
+        const int64_t last = it.first + it.tiles - tile + info.z - 1;  // its last tile on the line
+        p.joint[p.by_seq ? b : stretch] = make_int4(b, stretch, line.stretch_of(last, p.parts), 0);
       } else if (p.by_seq ? begins : info.y >> 1) {
         p.joint[p.by_seq ? b : stretch] = make_int4(-1, 0, 0, 0);
       }
     }
     opens = true;
-    tile = 0;
-    if (!(info.y >> 1)) {
-      ++b;
-      continue;
-    }
-    // ---- the next item
-    Item it;
-    for (item += warps; item < n_items; item += warps) {
-      it = item_at(item);
-      if (it.tiles > 0) break;
-    }
-    if (item >= n_items) break;
-    const Place at = start_of(it);
-    unit = it.unit, b = at.b, tile = at.tile;
-    if constexpr (C::kQRegs) {  // (what was fetched ahead is not it)
-      copies_landed();
-      __syncwarp();
-      fetch_q(b, unit);
-    }
+    if (next_item >= n_items) break;
+    item = next_item, unit = next_unit, b = next_b, tile = next_tile;
+    next_b = b + 1, next_tile = 0;
   }
   copies_landed();
   if (s_abort)  // a copy never came: those that are still under way are waited for, within limits
@@ -814,7 +868,6 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
 
 // Joins the sums of the sequences that go on.  A team of threads, four values each, adds up sums of a slice of a (sequence, head);
 // where there are many sums, they are dealt out to teams, and where there are few heads, these to slices.
-constexpr int kJoinThreads = 256;
 template <int DP, typename T, int BIAS, int AHEAD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ PagedParams p) {
   __shared__ float4 s_acc[kJoinThreads / 32][32];
@@ -829,9 +882,19 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int unit = hk * p.splits + split, m = h - hk * p.heads - split * p.rows;
   const int64_t step = 2ll * p.units * p.rows * row_floats(DP);  // from stretch to stretch
   const float* base = p.part + (static_cast<int64_t>(unit) * p.rows + m) * row_floats(DP);
+  int4 joint = make_int4(-1, 0, 0, 0);
+  if (!p.joint) {  // few sequences: by the lengths, while the sums are still being formed
+    const int lane = tid & 31, n = lane < p.B ? tiles_in<DP == 64 ? 32 : 16>(length_of(p, lane)) : 0;
+    const int64_t upto = warp_scan(n), tiles = __shfl_sync(0xffffffffu, upto, 31);
+    const Line line(tiles, p.ctas);
+    int from = 0, to = 0;
+    if (lane < p.B) from = line.stretch_of(upto - n, p.parts), to = line.stretch_of(upto - 1, p.parts);
+    joint = make_int4(which, __shfl_sync(0xffffffffu, from, which & 31), __shfl_sync(0xffffffffu, to, which & 31), 0);
+    if (which >= p.joints || joint.y == joint.z) joint.x = -1;
+  }
   grid_dep_wait();
   const int status = *reinterpret_cast<volatile int*>(p.status);
-  const int4 joint = which < p.joints ? __ldcg(p.joint + which) : make_int4(-1, 0, 0, 0);
+  if (p.joint && which < p.joints) joint = __ldcg(p.joint + which);
   if (status != 0) return;
   base += joint.y * step;
   const int n = joint.x < 0 ? 0 : joint.z - joint.y + 1;
@@ -895,18 +958,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
 }
 
-// How a call is cut: rows a unit, units a key head, warps, their ring, the grid.
-struct PagedPlan {
-  int DP, NQ, rows, splits, units;
-  int warps, ring, parts;
-  int ctas, joints, slices, teams, ahead;
-  bool whole, by_seq;
-};
-constexpr int kPagedSmem = 218 * 1024;  // shared memory for the warps' rooms
-
 template <int DP, int NQ, typename T, int BIAS, bool TILES>
 int launch_inst(const PagedParams& d, const PagedPlan& x, cudaStream_t stream) {
-  using C = Cfg<DP, NQ, TILES>;
+  using C = Cfg<DP, NQ>;
   static std::atomic<uint64_t> ready{0};  // devices whose kernel has its shared memory
   int dev = 0;
   cudaGetDevice(&dev);
@@ -941,7 +995,6 @@ int launch_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStr
     if (x.NQ == 4) return launch_bias<DP, 4, T, TILES>(d, x, bias_kind, stream);
   return launch_bias<DP, 2, T, TILES>(d, x, bias_kind, stream);
 }
-// The kernels of a type and a kind of copies; each such pair is a translation unit of its own.
 template <typename T, bool TILES>
 int launch_paged_kernels(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
   return x.DP == 256   ? launch_rows<256, T, TILES>(d, x, bias_kind, stream)
@@ -949,9 +1002,5 @@ int launch_paged_kernels(const PagedParams& d, const PagedPlan& x, int bias_kind
                        : launch_rows<64, T, TILES>(d, x, bias_kind, stream);
 }
 
-extern template int launch_paged_kernels<__nv_bfloat16, true>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
-extern template int launch_paged_kernels<__nv_bfloat16, false>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
-extern template int launch_paged_kernels<__half, true>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
-extern template int launch_paged_kernels<__half, false>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
-
+}  // namespace
 }  // namespace fa

@@ -2,5 +2,9 @@
 #include "fa_paged.cuh"
 
 namespace fa {
-template int launch_paged_kernels<__nv_bfloat16, false>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
+
+int launch_paged_bf16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
+  return launch_paged_kernels<__nv_bfloat16, false>(d, x, bias_kind, stream);
+}
+
 }  // namespace fa

@@ -2,5 +2,9 @@
 #include "fa_paged.cuh"
 
 namespace fa {
-template int launch_paged_kernels<__half, false>(const PagedParams&, const PagedPlan&, int, cudaStream_t);
+
+int launch_paged_f16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
+  return launch_paged_kernels<__half, false>(d, x, bias_kind, stream);
+}
+
 }  // namespace fa
