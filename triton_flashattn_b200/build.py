@@ -32,8 +32,10 @@ SOURCES = [
     "fa_small.cu",
     "fa_paged.cu",
     "fa_paged_bf16.cu",
+    "fa_paged_bf16_box8.cu",
     "fa_paged_bf16_rows.cu",
     "fa_paged_f16.cu",
+    "fa_paged_f16_box8.cu",
     "fa_paged_f16_rows.cu",
     "fa_kv.cu",
     "fa_copy.cu",

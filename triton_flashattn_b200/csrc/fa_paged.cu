@@ -60,7 +60,7 @@ uint64_t part_bytes(const PagedPlan& x) {
 }
 
 // Tile map of a cache.  False where its layout has none (an expanded view): then its rows are copied one by one.
-bool cache_map(CUtensorMap* out, const void* base, const fa_paged_params& p, const int64_t s[3]) {
+bool cache_map(CUtensorMap* out, const void* base, const fa_paged_params& p, const int64_t s[3], int box_keys) {
   const int extent[3] = {p.num_pages, p.page_size, p.Hkv};
   uint64_t bytes[3];
   for (int i = 0; i < 3; ++i) {
@@ -72,7 +72,7 @@ bool cache_map(CUtensorMap* out, const void* base, const fa_paged_params& p, con
   const uint64_t dims[4] = {static_cast<uint64_t>(p.D), static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.page_size),
                             static_cast<uint64_t>(p.num_pages)};
   const uint64_t strides[3] = {bytes[2], bytes[1], bytes[0]};
-  const uint32_t box[4] = {64, 1, 16, 1};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(box_keys), 1};
   return make_tmap_4d(out, base, 2, dims, strides, box) == FA_OK;
 }
 
@@ -85,7 +85,8 @@ uint64_t paged_workspace_bytes(const fa_paged_params& p) {
 
 int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream, int* status) {
   PagedParams d;
-  const bool aligned = p.page_size % 16 == 0 && cache_map(&d.k_map, p.k_cache, p, p.k_stride) && cache_map(&d.v_map, p.v_cache, p, p.v_stride);
+  int box = p.page_size % 16 == 0 ? 16 : p.page_size % 8 == 0 ? 8 : 0;
+  if (box && (!cache_map(&d.k_map, p.k_cache, p, p.k_stride, box) || !cache_map(&d.v_map, p.v_cache, p, p.v_stride, box))) box = 0;
   const PagedPlan x = plan_paged(p);
   d.q = p.q, d.k = p.k_cache, d.v = p.v_cache, d.bias = p.bias, d.o = p.o;
   d.table = p.block_table, d.lens = p.seq_lens, d.status = status;
@@ -96,7 +97,7 @@ int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream,
   d.v_sP = p.v_stride[0], d.v_sT = p.v_stride[1], d.v_sH = p.v_stride[2];
   d.bias_sB = p.bias_stride[0], d.bias_sH = p.bias_stride[1], d.table_s = p.table_stride;
   d.B = p.B, d.H = p.H, d.Hkv = p.Hkv, d.D = p.D;
-  d.page_size = p.page_size, d.num_pages = p.num_pages, d.width = p.width, d.page_tiles = p.page_size / 16;
+  d.page_size = p.page_size, d.num_pages = p.num_pages, d.width = p.width, d.page_boxes = box ? p.page_size / box : 0;
   d.heads = p.H / p.Hkv, d.rows = x.rows, d.splits = x.splits, d.units = x.units;
   d.parts = x.parts, d.ring = x.ring, d.whole = x.whole ? 1 : 0, d.by_seq = x.by_seq ? 1 : 0, d.joints = x.joints, d.ctas = x.ctas, d.slices = x.slices, d.teams = x.teams;
   d.scale = p.bias_kind == FA_BIAS_NONE || p.bias_kind == FA_BIAS_BOOL ? p.sm_scale * kLog2e : p.sm_scale;
@@ -107,10 +108,13 @@ int launch_paged(const fa_paged_params& p, void* workspace, cudaStream_t stream,
     shift = s;
     mul = static_cast<uint32_t>((((1ull << s) - by) << 32) / by + 1);
   };
-  divisor(aligned ? p.page_size / 16 : p.page_size, d.div_mul, d.div_shift);
+  divisor(box ? p.page_size / box : p.page_size, d.div_mul, d.div_shift);
   divisor(x.splits, d.splits_mul, d.splits_shift);
-  if (p.dtype == FA_BF16) return (aligned ? launch_paged_bf16_tiles : launch_paged_bf16_rows)(d, x, p.bias_kind, stream);
-  return (aligned ? launch_paged_f16_tiles : launch_paged_f16_rows)(d, x, p.bias_kind, stream);
+  const bool bf16 = p.dtype == FA_BF16;
+  PagedLaunch* launch = box == 16  ? (bf16 ? launch_paged_bf16 : launch_paged_f16)
+                        : box == 8 ? (bf16 ? launch_paged_bf16_box8 : launch_paged_f16_box8)
+                                   : (bf16 ? launch_paged_bf16_rows : launch_paged_f16_rows);
+  return launch(d, x, p.bias_kind, stream);
 }
 
 }  // namespace fa

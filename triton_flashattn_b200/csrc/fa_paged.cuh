@@ -6,7 +6,7 @@
 //
 // What bounds it: the keys and values are read once and each takes part in a handful of products (one for each query head that
 // shares it), so it is a stream from memory.  Each warp has a ring of tiles of 16 or 32 keys in shared memory that it fills itself,
-// by tile copies where pages are whole tiles and else by a copy for each row, and empties with the warp-level matrix
+// by tile copies where pages are whole boxes of 8 or 16 keys and else 16 bytes a lane, and empties with the warp-level matrix
 // instruction: the heads that share a key head are the 8, 16 or 32 columns of the product.  Its copies run ahead over the ends of
 // sequences and heads, so the stream does not stop there.
 //
@@ -24,7 +24,7 @@
 namespace fa {
 
 struct PagedParams {
-  CUtensorMap k_map, v_map;  // {D, Hkv, page_size, pages}, boxes of 64 elements and 16 tokens
+  CUtensorMap k_map, v_map;  // {D, Hkv, page_size, pages}, boxes of 64 elements and 8 or 16 tokens
   const void* q;
   const void* k;
   const void* v;
@@ -38,8 +38,8 @@ struct PagedParams {
                 // few sequences, where the joining kernel finds out itself, and where none goes on
   int64_t q_sB, q_sH, o_sB, o_sH, k_sP, k_sT, k_sH, v_sP, v_sT, v_sH, bias_sB, bias_sH, table_s;
   int B, H, Hkv, D;
-  int page_size, num_pages, width, page_tiles;
-  uint32_t div_mul, div_shift;        // division by the page size (in 16 keys where pages are whole tiles)
+  int page_size, num_pages, width, page_boxes;
+  uint32_t div_mul, div_shift;        // division by the page size (in boxes where pages are whole boxes)
   uint32_t splits_mul, splits_shift;  // by `splits`
   int heads;   // query heads of a key head
   int rows;    // of them, those of a unit
@@ -67,11 +67,10 @@ constexpr int kPagedSmem = 218 * 1024;  // shared memory for the warps' rooms
 // An unfinished sum: per row DP values, their maximum and the sum of the weights (and two words to keep rows at 16 bytes).
 __host__ __device__ constexpr int row_floats(int DP) { return DP + 4; }
 
-// The kernels of a type and a kind of copies, each pair in a translation unit of its own.
-int launch_paged_bf16_tiles(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
-int launch_paged_bf16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
-int launch_paged_f16_tiles(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
-int launch_paged_f16_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+// The kernels of a type and a kind of copies (boxes of 16 or 8 keys, or row by row), each in a translation unit of its own.
+using PagedLaunch = int(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream);
+PagedLaunch launch_paged_bf16, launch_paged_bf16_box8, launch_paged_bf16_rows;
+PagedLaunch launch_paged_f16, launch_paged_f16_box8, launch_paged_f16_rows;
 
 constexpr int kMostWarps = 8;
 // Up to this many sequences a lane has one, and the places of the sequences are known without tables.
@@ -231,11 +230,13 @@ __device__ __forceinline__ int tiles_in(int len) {
   return max((len + KEYS - 1) / KEYS, 1);
 }
 
-template <int DP, int NQ, typename T, int BIAS, bool TILES>
+template <int DP, int NQ, typename T, int BIAS, int BOX>
 __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_constant__ PagedParams p) {
   using P2 = Pack2<T>;
   using C = Cfg<DP, NQ>;
   constexpr int KS = DP / 16;  // steps of 16 head-dim elements
+  constexpr bool TILES = BOX > 0;
+  constexpr int kBoxes = TILES ? C::kKeys / BOX : 1;  // of a tile
   constexpr int MB = C::kPieces, kMostRing = 8;
   constexpr int kMostThreads = kMostWarps * 32;
 
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   // What no copy writes is read all the same, times 0: columns behind the head dim, rows of queries that the unit has not, keys
   // behind the last one or on no page.  (What an earlier tile left is as good as zeros; an infinite or NaN value would be put right, slowly.)
   {
-    const int from = TILES && MB == 1 ? 2 * S * C::kTile : 0;
+    const int from = kBoxes == 1 && TILES ? 2 * S * C::kTile : 0;
     for (int i = from / 16 + lane; i < (2 * S * C::kTile + C::kQ) / 16; i += 32)
       reinterpret_cast<uint4*>(room)[i] = make_uint4(0, 0, 0, 0);
   }
@@ -386,13 +387,14 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
 
   // ---- the copies, ahead of the products.  Pages: lane l knows that of the 16 keys (TILES; else of the key) number l of the
   // batch that begins at tile `batch` of sequence i_b, and the same of the batch after that.
-  constexpr int kBatch = TILES ? 32 / MB : 1;  // tiles
+  constexpr int kBatch = TILES ? 32 / kBoxes : 1;  // tiles
   const auto fetch_pages = [&](int b, int tile) {
-    const int what = TILES ? tile * MB + lane : tile * C::kKeys + (lane & (C::kKeys - 1));
+    const int what = TILES ? tile * kBoxes + lane : tile * C::kKeys + (lane & (C::kKeys - 1));
     const int at_page = fast_div(what, p.div_mul, p.div_shift);
-    const int id = b < p.B && at_page < p.width ? __ldcg(p.table + b * p.table_s + at_page) : -1;
-    return id >= 0 && id < p.num_pages ? id : -1;
+    return b < p.B && at_page < p.width ? __ldcg(p.table + b * p.table_s + at_page) : -1;
   };
+  // (looked at only when it is needed: nothing waits for a batch that is fetched ahead)
+  const auto in_cache = [&](int id) { return id >= 0 && id < p.num_pages ? id : -1; };
   int i_item = warp, i_unit = 0, i_head = 0;  // of the next tile to be copied: its item, ...
   int64_t i_left = 0;                         // tiles of the item that are not copied yet, it among them
   int i_b = 0, i_tile = 0, i_len = 0, i_tiles = 0;
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
         i_head = fast_div(i_unit, p.splits_mul, p.splits_shift);
         i_b = at.b, i_tile = at.tile, i_len = at.len, i_tiles = tiles_of(at.len);
         batch = i_tile / kBatch * kBatch;
-        page_l = fetch_pages(i_b, batch);
+        page_l = in_cache(fetch_pages(i_b, batch));
         fetch_next();
         return;
       }
@@ -436,13 +438,13 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
 
   // The next tile: its key head, pages and first rows there (TILES: of each piece; else of the lane's key), its keys, and whether
   // it is the last one.
-  int t_head = 0, t_page[TILES ? MB : 1], t_row[TILES ? MB : 1];
+  int t_head = 0, t_page[kBoxes], t_row[kBoxes];
   uint32_t t_keys = 0, t_last = 0, t_tiles = 0;
   int t_rows = 0;      // with a bias: rows of its unit,
   int64_t t_bias = 0;  // and where theirs begins
   const auto turn_to_next = [&] {
     if (i_tile - batch >= kBatch || i_tile < batch) {
-      batch = next_batch, page_l = next_page;
+      batch = next_batch, page_l = in_cache(next_page);
       fetch_next();
     }
     t_head = i_head;
@@ -450,11 +452,11 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     t_keys = behind >= C::kKeys ? 0xffffffffu >> (32 - C::kKeys) : (1u << max(behind, 0)) - 1u;
     if constexpr (TILES) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const int piece = i_tile * MB + i;
-        t_page[i] = __shfl_sync(0xffffffffu, page_l, piece - batch * MB);
-        t_row[i] = (piece - fast_div(piece, p.div_mul, p.div_shift) * p.page_tiles) * 16;
-        if (t_page[i] < 0) t_keys &= ~(0xffffu << (16 * i));
+      for (int i = 0; i < kBoxes; ++i) {
+        const int box = i_tile * kBoxes + i;
+        t_page[i] = __shfl_sync(0xffffffffu, page_l, box - batch * kBoxes);
+        t_row[i] = (box - fast_div(box, p.div_mul, p.div_shift) * p.page_boxes) * BOX;
+        if (t_page[i] < 0) t_keys &= ~(0xffffffffu >> (32 - BOX) << (BOX * i));
       }
     } else {
       const int key = i_tile * C::kKeys + (lane & (C::kKeys - 1));
@@ -487,15 +489,19 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     if constexpr (TILES) {
       if (elect_one()) {
         s_info[warp][to] = make_uint4(t_keys, t_last, t_tiles, 0);
-        // (a piece without a key is left out: what lies there, finite or not, counts for nothing)
-        mbar_expect_tx(&full[to], MB == 2 && t_keys >> 16 ? 4 * C::kPiece : 2 * C::kPiece);
+        // (a box without a key is left out: what lies there, finite or not, counts for nothing)
+        int boxes = 1;
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-          if (i == 0 || t_keys >> 16) {
+        for (int i = 1; i < kBoxes; ++i) boxes += t_keys >> (BOX * i) ? 1 : 0;
+        mbar_expect_tx(&full[to], boxes * (2 * BOX * 2 * DP));
+#pragma unroll
+        for (int i = 0; i < kBoxes; ++i)
+          if (i < boxes) {
+            const uint32_t at = (i * BOX >> 4) * C::kPiece + (i * BOX & 15) * 128;
 #pragma unroll
             for (int g = 0; g < DP / 64; ++g) {
-              tma_load_4d_to(k_dst + i * C::kPiece + g * 2048, &p.k_map, &full[to], g * 64, t_head, t_row[i], t_page[i]);
-              tma_load_4d_to(v_dst + i * C::kPiece + g * 2048, &p.v_map, &full[to], g * 64, t_head, t_row[i], t_page[i]);
+              tma_load_4d_to(k_dst + at + g * 2048, &p.k_map, &full[to], g * 64, t_head, t_row[i], t_page[i]);
+              tma_load_4d_to(v_dst + at + g * 2048, &p.v_map, &full[to], g * 64, t_head, t_row[i], t_page[i]);
             }
           }
       }
@@ -958,7 +964,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
 }
 
-template <int DP, int NQ, typename T, int BIAS, bool TILES>
+template <int DP, int NQ, typename T, int BIAS, int BOX>
 int launch_inst(const PagedParams& d, const PagedPlan& x, cudaStream_t stream) {
   using C = Cfg<DP, NQ>;
   static std::atomic<uint64_t> ready{0};  // devices whose kernel has its shared memory
@@ -966,12 +972,12 @@ int launch_inst(const PagedParams& d, const PagedPlan& x, cudaStream_t stream) {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return FA_ERR_CUDA;
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(paged_kernel<DP, NQ, T, BIAS, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem + 1024) != cudaSuccess)
+    if (cudaFuncSetAttribute(paged_kernel<DP, NQ, T, BIAS, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem + 1024) != cudaSuccess)
       return FA_ERR_CUDA;
     ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   const int smem = x.warps * C::warp_bytes(x.ring) + 1024;
-  if (int e = launch_overlapped(paged_kernel<DP, NQ, T, BIAS, TILES>, dim3(x.ctas), x.warps * 32, smem, stream, d)) return e;
+  if (int e = launch_overlapped(paged_kernel<DP, NQ, T, BIAS, BOX>, dim3(x.ctas), x.warps * 32, smem, stream, d)) return e;
   if (x.whole) return FA_OK;
   const int per_block = kJoinThreads / (DP / 4 / x.slices * x.teams);
   const int64_t blocks = (static_cast<int64_t>(x.joints) * d.H * x.slices + per_block - 1) / per_block;
@@ -979,27 +985,27 @@ int launch_inst(const PagedParams& d, const PagedPlan& x, cudaStream_t stream) {
                       : launch_overlapped(join_kernel<DP, T, BIAS, 8>, dim3(static_cast<unsigned>(blocks)), kJoinThreads, 0, stream, d);
 }
 
-template <int DP, int NQ, typename T, bool TILES>
+template <int DP, int NQ, typename T, int BOX>
 int launch_bias(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
   switch (bias_kind) {
-    case FA_BIAS_NONE: return launch_inst<DP, NQ, T, FA_BIAS_NONE, TILES>(d, x, stream);
-    case FA_BIAS_SAME: return launch_inst<DP, NQ, T, FA_BIAS_SAME, TILES>(d, x, stream);
-    case FA_BIAS_BOOL: return launch_inst<DP, NQ, T, FA_BIAS_BOOL, TILES>(d, x, stream);
-    default: return launch_inst<DP, NQ, T, FA_BIAS_F32, TILES>(d, x, stream);
+    case FA_BIAS_NONE: return launch_inst<DP, NQ, T, FA_BIAS_NONE, BOX>(d, x, stream);
+    case FA_BIAS_SAME: return launch_inst<DP, NQ, T, FA_BIAS_SAME, BOX>(d, x, stream);
+    case FA_BIAS_BOOL: return launch_inst<DP, NQ, T, FA_BIAS_BOOL, BOX>(d, x, stream);
+    default: return launch_inst<DP, NQ, T, FA_BIAS_F32, BOX>(d, x, stream);
   }
 }
-template <int DP, typename T, bool TILES>
+template <int DP, typename T, int BOX>
 int launch_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
-  if (x.NQ == 1) return launch_bias<DP, 1, T, TILES>(d, x, bias_kind, stream);
+  if (x.NQ == 1) return launch_bias<DP, 1, T, BOX>(d, x, bias_kind, stream);
   if constexpr (DP < 256)
-    if (x.NQ == 4) return launch_bias<DP, 4, T, TILES>(d, x, bias_kind, stream);
-  return launch_bias<DP, 2, T, TILES>(d, x, bias_kind, stream);
+    if (x.NQ == 4) return launch_bias<DP, 4, T, BOX>(d, x, bias_kind, stream);
+  return launch_bias<DP, 2, T, BOX>(d, x, bias_kind, stream);
 }
-template <typename T, bool TILES>
+template <typename T, int BOX>
 int launch_paged_kernels(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
-  return x.DP == 256   ? launch_rows<256, T, TILES>(d, x, bias_kind, stream)
-         : x.DP == 128 ? launch_rows<128, T, TILES>(d, x, bias_kind, stream)
-                       : launch_rows<64, T, TILES>(d, x, bias_kind, stream);
+  return x.DP == 256   ? launch_rows<256, T, BOX>(d, x, bias_kind, stream)
+         : x.DP == 128 ? launch_rows<128, T, BOX>(d, x, bias_kind, stream)
+                       : launch_rows<64, T, BOX>(d, x, bias_kind, stream);
 }
 
 }  // namespace

@@ -1,10 +1,10 @@
-// The paged attention kernels for fp16, tile copies.
+// The paged attention kernels for fp16, keys copied in boxes of 16 keys.
 #include "fa_paged.cuh"
 
 namespace fa {
 
-int launch_paged_f16_tiles(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
-  return launch_paged_kernels<__half, true>(d, x, bias_kind, stream);
+int launch_paged_f16(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
+  return launch_paged_kernels<__half, 16>(d, x, bias_kind, stream);
 }
 
 }  // namespace fa
