@@ -239,3 +239,17 @@ def test_cache_tensors():
     assert c.block_table.shape == (5, 3) and c.seq_lens.shape == (5,) and c.free_count.tolist() == [7]
     assert sorted(c.free_pages.tolist()) == list(range(7))
     assert all(t.dtype == torch.int32 for t in (c.block_table, c.seq_lens, c.free_pages, c.free_count))
+
+
+def test_operators_are_registered_with_shape_only_implementations():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops = torch.ops.triton_flashattn_b200
+    with FakeTensorMode():
+        q = torch.empty(2, 8, 64, dtype=BF, device="cuda")
+        cache = torch.empty(9, 16, 2, 64, dtype=BF, device="cuda")
+        table, lens = torch.empty(2, 4, dtype=torch.int32, device="cuda"), torch.empty(2, dtype=torch.int32, device="cuda")
+        out = ops.paged_attn(q, cache, cache, table, lens, None, 0.125)
+        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+        rows = torch.empty(5, 2, 64, dtype=BF, device="cuda")
+        assert ops.paged_kv_write(rows, rows, cache, cache, torch.empty(5, dtype=torch.int64, device="cuda")) is None

@@ -145,7 +145,8 @@ def test_attention_with_a_bias(lens, page, Hkv, group, D, dtype, kind, device_ok
 
 
 @pytest.mark.parametrize("lens,page,Hkv,group,D,dtype", [([100, 1, 777, 0], 16, 2, 4, 128, BF), ([130, 55], 24, 1, 10, 64, HF),
-                                                         ([300, 20], 32, 2, 2, 256, BF), ([90, 400], 5, 2, 3, 32, HF)])
+                                                         ([300, 20], 32, 2, 2, 256, BF), ([90, 400], 5, 2, 3, 32, HF),
+                                                         ([40, 210], 8, 1, 20, 128, BF), ([75, 130], 16, 1, 30, 64, HF)])
 @pytest.mark.parametrize("form", ["bool", "inf", "lowest"])
 def test_masks_and_what_hides_behind_them(lens, page, Hkv, group, D, dtype, form, device_ok):
     """Each head leaves out keys of its own, one head all of them, one head all but one; behind keys that every head leaves
@@ -303,6 +304,72 @@ def test_splits_of_many_and_of_long_sequences(B, longest, device_ok):
     check(got, q, kc, vc, table, n)
     for _ in range(3):
         assert torch.equal(fa.paged_attention_fn(q, kc, vc, table, n), got)
+
+
+@pytest.mark.parametrize("most_ctas", ["1", "3", "20"])
+@pytest.mark.parametrize("lens,page,Hkv,group,D", [([900, 0, 33, 2000], 16, 2, 4, 128), ([70] * 40, 8, 3, 2, 64),
+                                                   ([500, 1200, 1], 20, 1, 10, 256), ([5, 700] * 30, 16, 8, 1, 32)])
+def test_stretches_of_any_length(lens, page, Hkv, group, D, most_ctas, monkeypatch, device_ok):
+    """With one, three and twenty CTAs: long stretches over many sequences, more sequences than stretches and fewer."""
+    kc, vc, table, n = make_cache(lens, page, Hkv, D, BF, 15)
+    q = make_q(len(lens), Hkv * group, D, BF, 15)
+    monkeypatch.setenv("FA_MAX_CTAS", most_ctas)
+    check(fa.paged_attention_fn(q, kc, vc, table, n), q, kc, vc, table, n)
+
+
+@pytest.mark.parametrize("Hkv,group,D,longest", [(1, 3, 256, 20000), (8, 2, 128, 9000), (1, 20, 128, 6000), (5, 1, 16, 15000),
+                                                 (1, 32, 64, 8000)])
+def test_one_long_sequence(Hkv, group, D, longest, device_ok):
+    """Hundreds of unfinished sums a head, of every width, for the joining kernel."""
+    kc, vc, table, n = make_cache([longest], 16, Hkv, D, HF, 16)
+    q = make_q(1, Hkv * group, D, HF, 16)
+    check(fa.paged_attention_fn(q, kc, vc, table, n), q, kc, vc, table, n)
+
+
+def test_caches_that_are_expanded_views(device_ok):
+    """One page for all, one head for all: no tile map has them."""
+    g = torch.Generator().manual_seed(17)
+    page = torch.randn(1, 16, 2, 64, generator=g).to(BF).cuda()
+    kc, vc = page.expand(5, 16, 2, 64), (page[:, :, :1] * 2).expand(5, 16, 2, 64)
+    table, n = torch.tensor([[4, 0, 2]], dtype=torch.int32, device="cuda"), torch.tensor([41], dtype=torch.int32, device="cuda")
+    q = make_q(1, 4, 64, BF, 17)
+    check(fa.paged_attention_fn(q, kc, vc, table, n), q, kc, vc, table, n)
+
+
+def test_inference_mode_and_no_grad(device_ok):
+    with torch.inference_mode():
+        kc, vc, table, n = make_cache([30, 5], 16, 1, 64, BF, 18)
+        q = make_q(2, 2, 64, BF, 18)
+        out = fa.paged_attention_fn(q, kc, vc, table, n)
+        fa.paged_kv_write(kc[0, :2], vc[0, :2], kc, vc, torch.tensor([17, -1], device="cuda"))
+    with torch.no_grad():
+        kc, vc, table, n = make_cache([30, 5], 16, 1, 64, BF, 18)
+        assert torch.equal(fa.paged_attention_fn(make_q(2, 2, 64, BF, 18).requires_grad_(), kc, vc, table, n), out)
+    with pytest.raises(NotImplementedError):
+        fa.paged_attention_fn(make_q(2, 2, 64, BF, 18).requires_grad_(), kc, vc, table, n)
+
+
+def test_operators_are_captured_as_graph_nodes(device_ok):
+    kc, vc, table, n = make_cache([30, 65], 16, 2, 64, BF, 19, stale=0.0)
+    q, rows = make_q(2, 4, 64, BF, 19), make_q(2, 2, 64, BF, 20)
+    slots = torch.tensor([table[0, 0].item() * 16 + 3, -1], device="cuda")
+    k2, v2 = kc.clone(), vc.clone()
+    fa.paged_kv_write(rows, rows, kc, vc, slots)
+    want = fa.paged_attention_fn(q, kc, vc, table, n)
+    seen = []
+
+    def backend(gm, example_inputs):
+        seen.append([node.target for node in gm.graph.nodes if node.op == "call_function"])
+        return gm.forward
+
+    def step(q, rows, k, v):
+        fa.paged_kv_write_op(rows, rows, k, v, slots)
+        return fa.paged_attention_op(q, k, v, table, n)
+
+    with torch.no_grad():
+        out = torch.compile(step, backend=backend, fullgraph=True)(q, rows, k2, v2)
+    assert torch.equal(out, want) and torch.equal(k2, kc) and torch.equal(v2, vc)
+    assert any(torch.ops.triton_flashattn_b200.paged_attn.default in g for g in seen)
 
 
 def test_one_token_and_pages_shared_by_sequences(device_ok):

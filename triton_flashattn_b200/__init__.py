@@ -5,7 +5,8 @@ Public interface (same names and signatures as the reference project):
     FlashAttentionFn, FlashAttentionQKVPackedFn
 plus, with no counterpart in the reference: FlashAttention (nn.Module), flash_attention_op
 (the same call through torch.library operators), shard_batch_heads, and for serving a paged key / value
-cache: PagedKVCache, paged_attention_fn, paged_kv_extend, paged_kv_write, paged_kv_release.
+cache: PagedKVCache, paged_attention_fn, paged_kv_extend, paged_kv_write, paged_kv_release (and
+paged_attention_op, paged_kv_write_op through torch.library).
 """
 from .flash_attention import (  # noqa: F401
     FlashAttentionFn,
@@ -13,7 +14,7 @@ from .flash_attention import (  # noqa: F401
     flash_attention_fn,
     flash_attention_qkvpacked_fn,
 )
-from .module import FlashAttention, flash_attention_op  # noqa: F401
+from .module import FlashAttention, flash_attention_op, paged_attention_op, paged_kv_write_op  # noqa: F401
 from .paged import (  # noqa: F401
     PagedKVCache,
     paged_attention_fn,
@@ -33,7 +34,9 @@ __all__ = [
     "shard_batch_heads",
     "PagedKVCache",
     "paged_attention_fn",
+    "paged_attention_op",
     "paged_kv_extend",
     "paged_kv_release",
     "paged_kv_write",
+    "paged_kv_write_op",
 ]

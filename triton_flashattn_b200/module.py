@@ -6,6 +6,8 @@
   per direction instead of tracing into ctypes.
 * ``flash_attention_op``: same call signature and results as ``flash_attention_fn``, routed
   through those operators.
+* ``torch.ops.triton_flashattn_b200.paged_attn`` / ``paged_kv_write``: the two paged-cache calls of a
+  model's layer in the same form, and ``paged_attention_op`` / ``paged_kv_write_op`` that make them.
 * ``FlashAttention``: an ``nn.Module`` holding ``causal`` / ``sm_scale``.
 
 The reference project has no counterpart (it imports ``torch.nn`` but defines no module,
@@ -19,6 +21,7 @@ import torch
 from torch import nn
 
 from . import flash_attention as _fa
+from . import paged as _paged
 
 _NS = "triton_flashattn_b200"
 
@@ -80,6 +83,41 @@ def flash_attention_op(q, k, v, bias=None, causal=False, sm_scale=None):
     scale = float(q.shape[-1] ** -0.5 if sm_scale is None else sm_scale)
     out, _ = attn_fwd(q, k, v, bias, bool(causal), scale)
     return out
+
+
+@torch.library.custom_op(f"{_NS}::paged_attn", mutates_args=(), device_types="cuda")
+def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+               seq_lens: torch.Tensor, bias: Optional[torch.Tensor], sm_scale: float) -> torch.Tensor:
+    """(B, H, D) of the paged attention kernels."""
+    return _paged.paged_attention_fn(q, k_cache, v_cache, block_table, seq_lens, bias, sm_scale)
+
+
+@paged_attn.register_fake
+def _paged_attn_fake(q, k_cache, v_cache, block_table, seq_lens, bias, sm_scale):
+    return q.new_empty(tuple(q.shape))
+
+
+@torch.library.custom_op(f"{_NS}::paged_kv_write", mutates_args=("k_cache", "v_cache"), device_types="cuda")
+def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   slot_mapping: torch.Tensor) -> None:
+    """Rows into the caches, in place."""
+    _paged.paged_kv_write(k, v, k_cache, v_cache, slot_mapping)
+
+
+@paged_kv_write.register_fake
+def _paged_kv_write_fake(k, v, k_cache, v_cache, slot_mapping):
+    return None
+
+
+def paged_attention_op(q, k_cache, v_cache, block_table, seq_lens, bias=None, sm_scale=None):
+    """`paged_attention_fn` through the registered operator (graph-capture friendly)."""
+    scale = float(q.shape[-1] ** -0.5 if sm_scale is None else sm_scale)
+    return paged_attn(q, k_cache, v_cache, block_table, seq_lens, bias, scale)
+
+
+def paged_kv_write_op(k, v, k_cache, v_cache, slot_mapping):
+    """`paged_kv_write` through the registered operator (graph-capture friendly)."""
+    paged_kv_write(k, v, k_cache, v_cache, slot_mapping)
 
 
 class FlashAttention(nn.Module):
