@@ -5,20 +5,25 @@
 namespace fa {
 namespace {
 
-// Sequences of at most this many keys are not split over CTAs: one launch less.
+// Sequences of at most this many keys are not split over CTAs: one launch less.  Whole / split, us: one of 48 keys 7.0 / 6.7, 64 of up
+// to 48 9.4 / 10.3; one of 96 9.6 / 6.9, 64 of up to 100 13.1 / 13.9.
 constexpr int kWholeKeys = 64;
 
 PagedPlan plan_paged(const fa_paged_params& p) {
   PagedPlan x;
   const int heads = p.H / p.Hkv;
   x.DP = padded_head_dim(p.D);
-  x.NQ = heads <= 8 ? 1 : heads <= 16 || x.DP == 256 ? 2 : 4;
+  // Rows of a unit in groups of 8.  More heads than two groups are more units, which read the same keys side by side.
+  // 16 sequences of 1000 to 8000 keys, 4 key heads, one group / two, us: 16 heads each 41 / 38.6 (D 64, 32 sequences 43 / 37); 32 heads
+  // each 76 / 52, with four groups 56.
+  x.NQ = heads <= 8 ? 1 : 2;
   x.splits = (heads + 8 * x.NQ - 1) / (8 * x.NQ);
   x.rows = (heads + x.splits - 1) / x.splits;
   x.units = p.Hkv * x.splits;
   const int tile = (x.DP == 64 ? 2 : 1) * 32 * x.DP, queries = 8 * x.NQ * x.DP * 2;  // bytes, as Cfg has them
   // Warps: as many as there is room for, fewer where that spares parts (each has units / gcd items over 1 / parts of the
-  // stretch: a warp a unit, or some units, or some warps a unit).
+  // stretch: a warp a unit, or some units, or some warps a unit).  Always the most: two units at head dim 256 (5 warps for 4) 28 -> 40
+  // us, one unit at 128 (8 for 5) 24 -> 29.
   const auto ring_of = [&](int warps) { return ((kPagedSmem / warps) / 1024 * 1024 - queries) / (2 * tile); };
   int most = kMostWarps;
   while (most > 4 && ring_of(most) < 2) --most;

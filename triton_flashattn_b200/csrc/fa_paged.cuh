@@ -7,8 +7,9 @@
 // What bounds it: the keys and values are read once and each takes part in a handful of products (one for each query head that
 // shares it), so it is a stream from memory.  Each warp has a ring of tiles of 16 or 32 keys in shared memory that it fills itself,
 // by tile copies where pages are whole boxes of 8 or 16 keys and else 16 bytes a lane, and empties with the warp-level matrix
-// instruction: the heads that share a key head are the 8, 16 or 32 columns of the product.  Its copies run ahead over the ends of
-// sequences and heads, so the stream does not stop there.
+// instruction: the heads that share a key head are the 8 or 16 columns of the product.  Its copies run ahead over the ends of
+// sequences and heads, so the stream does not stop there.  (tcgen05 would want 128 rows of queries where there are 4 or 8, and
+// a hand-off between warps for every tile; a tile's 40 products take a tenth of the time that its bytes do.)
 //
 // Lengths are on the device and differ, and one long sequence must fill the SMs as well as thousands of short ones: the tiles of
 // all sequences, in order, are one line, and each CTA takes an equal stretch of it with all key heads, a warp one head (or one
@@ -16,6 +17,14 @@
 // time, which in a (page, token, head, element) cache are neighbours in memory.  A warp writes the sequences that lie whole in
 // its stretch; of the others, at most two, it leaves the unfinished sums in the workspace, where a second kernel joins them in
 // order.
+//
+// Measured, bf16, head dim 128, 32 query and 8 key heads, us (of the rate of a copy, 6453 GB/s):
+//   64 sequences of 200 to 8192 keys 177 (1.07 GB, 0.94), one of 131072 91 (0.91), one of 20011 24 (0.52), one of 1000 8.3
+// of which 5 pass before the first tile is there (lengths, pages, keys: one waits for the other) and 4 to 5 after the last one (the
+// second kernel).  In a large call 24 of the 148 SMs take 15 % longer than the others for the same bytes.
+//   What the forms before this one took, for the 64 sequences and the one of 20011: tiles in registers and one head a warp and
+//   stretch 190, 26; a ring, one head a warp and stretch 186, 25.  Four times as many, smaller stretches than CTAs fit: 200; a sixth
+//   of the line in small stretches for those who are done first: 180 to 188.
 #pragma once
 
 #include "fa_common.cuh"
@@ -177,7 +186,8 @@ __device__ __forceinline__ float bias_of(uint32_t x) {
   return BIAS == 3 ? __uint_as_float(x) : Pack2<T>::unpack(x).x;
 }
 
-// Shared memory of a kernel.  DP: head dim rounded up to 64, 128, 256; NQ: groups of 8 rows.
+// Shared memory of a kernel.  DP: head dim rounded up to 64, 128, 256; NQ: groups of 8 rows.  Tiles of 32 keys at DP 64: a tile
+// costs a warp 1000 cycles whatever its width (waits, votes, the maximum), as much as 4 KB take of the memory rate.
 template <int DP, int NQ>
 struct Cfg {
   static constexpr int kPieces = DP == 64 ? 2 : 1;  // of 16 keys, in a tile: what a warp waits for and works on at once
@@ -997,8 +1007,6 @@ int launch_bias(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStr
 template <int DP, typename T, int BOX>
 int launch_rows(const PagedParams& d, const PagedPlan& x, int bias_kind, cudaStream_t stream) {
   if (x.NQ == 1) return launch_bias<DP, 1, T, BOX>(d, x, bias_kind, stream);
-  if constexpr (DP < 256)
-    if (x.NQ == 4) return launch_bias<DP, 4, T, BOX>(d, x, bias_kind, stream);
   return launch_bias<DP, 2, T, BOX>(d, x, bias_kind, stream);
 }
 template <typename T, int BOX>
