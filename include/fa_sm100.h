@@ -1,7 +1,8 @@
 /*
  * C ABI of libfa_sm100.so: flash-attention forward and backward for NVIDIA B200
  * (sm_100a), with an optional (B,H,M,N) additive bias / bool mask and a bias
- * gradient written at full size.
+ * gradient written at full size; and, for serving, attention of single new tokens
+ * over a paged key / value cache, with the cache's upkeep.
  *
  * Every entry point takes plain pointers and sizes, enqueues work on the CUDA
  * stream it is given, never synchronises the device (except where noted), never
@@ -10,7 +11,8 @@
  * (fa_status_string() turns it into text).
  *
  * The entry points replace, one for one, the host launchers of the reference
- * project's flash_attention.py (cited per function below as FA:<line>).
+ * project's flash_attention.py (cited per function below as FA:<line>); those of the
+ * paged cache have no counterpart there.
  */
 #ifndef FA_SM100_H_
 #define FA_SM100_H_
@@ -116,7 +118,8 @@ int fa_version(void);
 
 /*
  * Number of kernels this library has launched since it was loaded (forward 1 per call; backward 3:
- * preprocess, dK/dV, dQ, with more parts two more each, or 1 where it is one launch (see fa_bwd); a row copy 1).  For
+ * preprocess, dK/dV, dQ, with more parts two more each, or 1 where it is one launch (see fa_bwd); a row copy 1; fa_paged_fwd 2, or
+ * 1 where no sequence is split; fa_kv_* 1).  For
  * benchmarks and tests that must show the work ran here.  No counterpart in the reference.
  */
 uint64_t fa_launch_count(void);
@@ -220,7 +223,7 @@ int fa_bwd_dq(const fa_params* p, void* stream);   /* _attn_bwd_dq         FA:53
  * A cache is num_pages pages of page_size tokens of Hkv heads: element (page, token, head, d) of k_cache and v_cache lies at
  * page * stride[0] + token * stride[1] + head * stride[2] + d.  Row b of block_table names the pages of sequence b in order;
  * the key at position n of it is token n % page_size of page block_table[b][n / page_size].  Entries behind the last page
- * of a sequence are not read.
+ * of a sequence may be read and are not used.
  */
 
 /*
