@@ -245,6 +245,21 @@ def test_lengths_and_pages_that_are_wrong(device_ok):
     assert not fa.paged_attention_fn(q, kc, vc, table, n).any()
 
 
+@pytest.mark.parametrize("page", [8, 20, 1])
+@pytest.mark.parametrize("D", [32, 128])
+def test_wrong_pages_of_other_sizes(page, D, device_ok):
+    """The same for pages that other copies bring: sequences without a key, pages that are not there first, last and between."""
+    kc, vc, table, n = make_cache([64, 64, 0, 41, 64], page, 2, D, HF, 7, width=80)
+    q = make_q(5, 6, D, HF, 7)
+    n[2] = -3
+    table[0, 0], table[1, 1], table[1, 2] = -1, kc.shape[0], 2 ** 31 - 1
+    table[3, (41 - 1) // page] = -2 ** 31
+    table[4] = -1
+    got = fa.paged_attention_fn(q, kc, vc, table, n)
+    check(got, q, kc, vc, table, n)
+    assert not got[2].any() and not got[4].any()
+
+
 @pytest.mark.parametrize("layout", ["heads_first", "layer", "padded", "token_first"])
 def test_cache_layouts(layout, device_ok):
     lens, page, Hkv, D = [100, 300, 5], 16, 2, 64

@@ -58,7 +58,7 @@ struct PagedParams {
   int ring;    // tiles that a warp has room for
   int whole;   // stretches are whole sequences
   int ctas;    // of the first kernel
-  int by_seq;  // joint has an entry for each sequence (else for each stretch)
+  int by_seq;  // joint has an entry for each sequence (else for each stretch: there are more sequences, so none is empty)
   int joints;  // entries of it
   int slices, teams;  // of a (sequence, head) in the joining kernel
   float scale;  // of the scores; in log2 units unless there is a float bias
@@ -324,10 +324,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
   if (status != 0) return;
   const Line line(tiles, gridDim.x);
   const int me = blockIdx.x;
-  if (me >= line.ctas) {
-    if (p.joint && !p.by_seq && tid < p.parts) p.joint[me * p.parts + tid] = make_int4(-1, 0, 0, 0);
-    return;
-  }
+  if (me >= line.ctas) return;
 
   // A place on the line: a sequence and a tile of it.
   struct Place {
@@ -437,11 +434,8 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
         fetch_next();
         return;
       }
-      if (!p.whole) {
-        const int stretch = me * p.parts + x.part;
-        if (lane < p.rows) *reinterpret_cast<float2*>(part_at(stretch, 0, x.unit) + lane * row_floats(DP) + DP) = make_float2(-INFINITY, 0.f);
-        if (lane == 0 && x.unit == 0 && p.joint && !p.by_seq) p.joint[stretch] = make_int4(-1, 0, 0, 0);
-      }
+      if (!p.whole && lane < p.rows)
+        *reinterpret_cast<float2*>(part_at(me * p.parts + x.part, 0, x.unit) + lane * row_floats(DP) + DP) = make_float2(-INFINITY, 0.f);
     }
   };
   open_item();
