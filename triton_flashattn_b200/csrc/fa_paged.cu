@@ -41,7 +41,8 @@ PagedPlan plan_paged(const fa_paged_params& p) {
   const int64_t cap = static_cast<int64_t>(p.width) * p.page_size;
   const int keys = x.DP == 64 ? 32 : 16;
   const int64_t most_ctas = p.B * ((cap + keys - 1) / keys);
-  x.ctas = persistent_grid(static_cast<int>(most_ctas < 1 << 30 ? most_ctas : 1 << 30));
+  const int sms = persistent_grid(1 << 30);
+  x.ctas = static_cast<int>(most_ctas < sms ? most_ctas : sms);
   x.whole = cap <= kWholeKeys;
   if (x.whole) x.parts = 1;
   const int stretches = x.ctas * x.parts;
@@ -50,7 +51,7 @@ PagedPlan plan_paged(const fa_paged_params& p) {
   // More teams while a team has several rounds of sums and the SMs room for them; of smaller slices where a block holds no more.
   x.ahead = x.by_seq ? 8 : 4;  // (elsewhere a sequence has two sums, rarely more)
   const int64_t sums = p.B < stretches ? stretches / p.B : 1;
-  const int64_t room_for = static_cast<int64_t>(persistent_grid(1 << 30)) * 2 * kJoinThreads;
+  const int64_t room_for = static_cast<int64_t>(sms) * 2 * kJoinThreads;
   int size = x.DP / 4;
   x.slices = x.teams = 1;
   while (sums > x.ahead * x.teams && static_cast<int64_t>(x.joints) * p.H * (x.DP / 4) * x.teams * 2 <= room_for &&
