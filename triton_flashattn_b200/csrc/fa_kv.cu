@@ -23,8 +23,9 @@ Divisor divisor(uint64_t d) {
 }
 
 // ---- rows into the pages -----------------------------------------------------------------------
-// A copy: what bounds it is the memory, read once, written once.  A thread moves 16 bytes of K and of V of kAhead tokens; all its
-// loads are under way before the first store.
+// A copy: what bounds it is the memory, read once, written once.  A thread moves 16 bytes of K and of V in kAhead places, and all its
+// loads are under way before the first store.  16384 rows of 8 x 128 (134 MB): 22.5 us, 0.92 of a copy's rate; with one place a thread
+// and 64-bit divisions 28.5.
 struct WriteParams {
   const uint16_t* k;
   const uint16_t* v;
@@ -81,8 +82,10 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WritePara
 // ---- tables ------------------------------------------------------------------------------------
 // All CTAs of a call look at all requests, kThreads at a time, and have the same running sums; what is written (pages, slots) is
 // shared out over their warps, a run of neighbours each, so that a lane looks for the request of its first one, and again only
-// where its next one is another's.  Where lens_out is lens or count_out is count, the CTAs are one cluster, with a barrier between looking and writing.
-// What bounds a call is latency: a launch, the lengths, the pages, the stores.
+// where its next one is another's.  Where lens_out is lens or count_out is count, the CTAs are one cluster, with a barrier between
+// looking and writing.
+// What bounds a call is latency: a launch, the lengths, the pages, the stores.  256 requests with a token each 4.8 us; prompts of 131 k
+// tokens 8.4 (40 with a search for each token and a cluster in any case); 131 k pages given back 5.4 (26).
 constexpr int kThreads = 512;
 
 struct TableParams {
