@@ -699,9 +699,14 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float y = s[g][k][i] * p.scale;
-          // a mask selects: whatever the score of a masked key is (infinite, NaN), it takes no part
-          if constexpr (BIAS == 2) y = bf[g][k][i] ? y : -INFINITY;
-          else if constexpr (BIAS != 0) y += bias_of<BIAS, T>(bf[g][k][i]);
+          // a mask selects, and so does a bias of -inf: whatever the score of a key that is left out is (infinite, NaN), it takes
+          // no part
+          if constexpr (BIAS == 2) {
+            y = bf[g][k][i] ? y : -INFINITY;
+          } else if constexpr (BIAS != 0) {
+            const float plus = bias_of<BIAS, T>(bf[g][k][i]);
+            y = plus == -INFINITY ? -INFINITY : y + plus;
+          }
           if (!(keys >> (k * 16 + r + 8 * (i >> 1)) & 1)) y = -INFINITY;
           s[g][k][i] = y;
           need = need || y > mx[g][i & 1] + 8.f;
