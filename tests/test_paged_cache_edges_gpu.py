@@ -1,4 +1,4 @@
-"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out."""
+"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative."""
 import pytest
 import torch
 
@@ -51,3 +51,48 @@ def test_a_bias_of_minus_infinity_leaves_out_any_key(lens, page, Hkv, group, D, 
     assert torch.equal(seen[:, :-1], others[:, :-1])
     for b, length in enumerate(lens):
         assert seen[b, -1].isnan().all() if length else not seen[b].any()
+
+
+# ---------------------------------------------------------------------------------- operators without a derivative
+def test_operators_refuse_what_would_lose_a_derivative(device_ok):
+    """Grad, functorch's grad and a tangent: refused before anything is written."""
+    kc, vc, table, n = make_cache([30, 5], 16, 1, 64, BF, 62, stale=0.0)
+    q, rows = make_q(2, 2, 64, BF, 62), make_q(2, 1, 64, BF, 63)
+    slots = torch.tensor([17, 3], device="cuda")
+    before = kc.clone(), vc.clone()
+    for wants in ((rows.clone().requires_grad_(), rows), (rows, rows.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError, match="no backward"):
+            fa.paged_kv_write_op(*wants, kc, vc, slots)
+        with pytest.raises(NotImplementedError, match="no backward"):
+            torch.ops.triton_flashattn_b200.paged_kv_write(*wants, kc, vc, slots)
+    for i in range(3):
+        a = [q, kc, vc]
+        a[i] = a[i].clone().requires_grad_()
+        with pytest.raises(NotImplementedError, match="no backward"):
+            fa.paged_attention_op(*a, table, n)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        fa.paged_attention_op(q, kc, vc, table, n, torch.zeros(2, 2, table.shape[1] * 16, device="cuda", requires_grad=True))
+
+    def through(k):
+        fa.paged_kv_write_op(k, rows, kc, vc, slots)
+        return kc.float().sum()
+
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.grad(through)(rows)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.grad(lambda q: fa.paged_attention_op(q, kc, vc, table, n).float().sum())(q)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(rows, rows)
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            fa.paged_kv_write_op(dual, rows, kc, vc, slots)
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            fa.paged_attention_op(torch.autograd.forward_ad.make_dual(q, q), kc, vc, table, n)
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+    with torch.no_grad():
+        leaf = rows.clone().requires_grad_()
+        version = kc._version
+        fa.paged_kv_write_op(leaf, leaf, kc, vc, slots)
+        assert kc._version > version and torch.equal(kc[1, 1], rows[0]) and torch.equal(vc[0, 3], rows[1])
+        want = fa.paged_attention_fn(q, kc, vc, table, n)
+        assert torch.equal(fa.paged_attention_op(q.clone().requires_grad_(), kc, vc, table, n), want)
+    assert torch.equal(fa.paged_attention_op(q, kc, vc, table, n), want)

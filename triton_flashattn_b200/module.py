@@ -8,6 +8,7 @@
   through those operators.
 * ``torch.ops.triton_flashattn_b200.paged_attn`` / ``paged_kv_write``: the two paged-cache calls of a
   model's layer in the same form, and ``paged_attention_op`` / ``paged_kv_write_op`` that make them.
+  Without a derivative: an input that requires grad is refused outside ``torch.no_grad()``.
 * ``FlashAttention``: an ``nn.Module`` holding ``causal`` / ``sm_scale``.
 
 The reference project has no counterpart (it imports ``torch.nn`` but defines no module,
@@ -107,6 +108,27 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
 @paged_kv_write.register_fake
 def _paged_kv_write_fake(k, v, k_cache, v_cache, slot_mapping):
     return None
+
+
+# The bodies above run with grad mode off, so the refusals in them never see that a gradient is wanted: the rows written would lose
+# theirs without a word, and the attention would fail only in its backward.  So the operators refuse before they dispatch.
+_lib = torch.library.Library(_NS, "FRAGMENT")
+
+
+def _refuse_gradients(name: str) -> None:
+    def refuse(*args, **kwargs):
+        if torch.is_grad_enabled():
+            for x in (*args, *kwargs.values()):
+                if isinstance(x, torch.Tensor) and x.requires_grad:
+                    raise NotImplementedError(f"{name} has no backward: call it under torch.no_grad()")
+        with torch._C._AutoDispatchBelowAutograd():
+            return getattr(getattr(torch.ops, _NS), name).default(*args, **kwargs)
+
+    _lib.impl(name, refuse, "AutogradCUDA")
+
+
+_refuse_gradients("paged_attn")
+_refuse_gradients("paged_kv_write")
 
 
 def paged_attention_op(q, k_cache, v_cache, block_table, seq_lens, bias=None, sm_scale=None):
