@@ -1,4 +1,5 @@
-"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative."""
+"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, scores at the end
+of what fp32 tells apart."""
 import pytest
 import torch
 
@@ -96,3 +97,17 @@ def test_operators_refuse_what_would_lose_a_derivative(device_ok):
         want = fa.paged_attention_fn(q, kc, vc, table, n)
         assert torch.equal(fa.paged_attention_op(q.clone().requires_grad_(), kc, vc, table, n), want)
     assert torch.equal(fa.paged_attention_op(q, kc, vc, table, n), want)
+
+
+# ---------------------------------------------------------------------------------- weights
+@pytest.mark.parametrize("first", [2.0 ** 27 + 16, -(2.0 ** 27 + 48)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_scores_so_large_that_fp32_steps_by_16(first, D, monkeypatch, device_ok):
+    """fp16 with an fp32 bias whose neighbours are 16 apart: the next score up has e^16 times the weight, beyond fp16, unless the
+    running maximum moves."""
+    monkeypatch.setenv("FA_MAX_CTAS", "1")
+    kc, vc, table, n = make_cache([1000], 16, 1, D, HF, 71)
+    q = torch.zeros(1, 3, D, dtype=HF, device="cuda")
+    pos = torch.arange(table.shape[1] * 16, device="cuda")
+    bias = (first + 16.0 * (pos // 32 % 2)).float().expand(1, 3, -1)
+    check(fa.paged_attention_fn(q, kc, vc, table, n, bias), q, kc, vc, table, n, bias)

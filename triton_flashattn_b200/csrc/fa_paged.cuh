@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           }
           if (!(keys >> (k * 16 + r + 8 * (i >> 1)) & 1)) y = -INFINITY;
           s[g][k][i] = y;
-          need = need || y > mx[g][i & 1] + 8.f;
+          need = need || y - mx[g][i & 1] > 8.f;  // (the difference that the weight is taken of: a sum may be rounded up by more)
         }
     if (BIAS != 0 && info.y == 0) load_b(tile + 1, s_info[warp][place + 1 == S ? 0 : place + 1].x);
     if (__any_sync(0xffffffffu, need)) {
