@@ -1,5 +1,5 @@
-"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, scores at the end
-of what fp32 tells apart."""
+"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, weights far below the
+largest one, scores at the end of what fp32 tells apart."""
 import pytest
 import torch
 
@@ -100,6 +100,54 @@ def test_operators_refuse_what_would_lose_a_derivative(device_ok):
 
 
 # ---------------------------------------------------------------------------------- weights
+@pytest.mark.parametrize("n,D,group,most_ctas", [(65536, 64, 4, "1"), (30011, 128, 1, "1"), (9000, 256, 12, "1"), (200000, 32, 2, "2")])
+@pytest.mark.parametrize("below", [12.3, 17.9, 20.6])
+@pytest.mark.parametrize("kind", ["none", "mask", "same", "f32"])
+def test_one_strong_key_and_many_weak_ones(n, D, group, most_ctas, below, kind, monkeypatch, device_ok):
+    """fp16: one key at the front, whose value is 0, and thousands whose weights are e^-below of its: what these add up to is all
+    there is in the result.
+
+    The tolerance, relative to sum w |v| (w the normalised weights): a score is exact up to its product with the scale and, with
+    no bias, log2 e, and so is the difference of two: 2^-22 (|s| + |max|); the exponential adds 2^-21, numerator and
+    sum have both: twice.  Sums of n keys in fp32, in both: 2 (n + 64) 2^-24.  Absolute: a weight enters the product in two fp16
+    terms, the second rounded to half of fp16's smallest step, 2^-25, in units of 2^-7 of a weight of 1, and weights are at least the
+    true ones beside the largest: 2^-32 a key over the sum of the weights; the result's own rounding 2^-11 relative, and not
+    below 2^-25."""
+    monkeypatch.setenv("FA_MAX_CTAS", most_ctas)
+    page = 16
+    pages = -(-n // page)
+    g = torch.Generator().manual_seed(70)
+    kc = torch.zeros(pages, page, 1, D, dtype=HF, device="cuda")
+    vc = torch.zeros(pages, page, 1, D, dtype=HF, device="cuda")
+    v = (1 + torch.rand(D, generator=g)).to(HF).cuda()
+    vc[:] = v
+    vc[0, 0] = 0.0
+    q = torch.zeros(1, group, D, dtype=HF, device="cuda")
+    q[:, :, 0] = 1.0
+    table = torch.randperm(pages - 1, generator=g).int()[None] + 1
+    table = torch.cat([torch.zeros(1, 1, dtype=torch.int32), table], 1).cuda()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    bias, scale = None, 1.0
+    if kind in ("none", "mask"):
+        kc[0, 0, 0, 0] = below  # (rounded to fp16: taken from there below)
+        gap = kc[0, 0, 0, 0].double().item()
+        if kind == "mask":
+            bias = torch.ones(1, 1, pages * page, dtype=torch.bool, device="cuda").expand(1, group, -1)
+    else:
+        row = torch.full((1, 1, pages * page), -below, dtype=HF if kind == "same" else torch.float32, device="cuda")
+        gap = -row[0, 0, 0].double().item()
+        row[:, :, 0] = 0.0
+        bias = row.expand(1, group, -1)
+    w = torch.exp(torch.tensor(-gap, dtype=torch.float64))
+    total = 1 + (n - 1) * w
+    share = (n - 1) * w / total  # sum w over the keys whose value is not 0
+    want = share * v.double().cpu()
+    rel = 2 * (2.0 ** -22 * 2 * gap + 2.0 ** -21) + 2 * (n + 64) * 2.0 ** -24
+    tol = (2.0 ** -11 + rel) * want + n * 2.0 ** -32 / total * v.double().cpu().max() + 2.0 ** -25
+    off = (fa.paged_attention_fn(q, kc, vc, table, lens, bias, scale)[0].double().cpu() - want).abs()
+    assert (off <= tol).all(), f"{(off / want).max().item():.3e} of the result, {(off / tol).max().item():.2f} of the tolerance"
+
+
 @pytest.mark.parametrize("first", [2.0 ** 27 + 16, -(2.0 ** 27 + 48)])
 @pytest.mark.parametrize("D", [64, 256])
 def test_scores_so_large_that_fp32_steps_by_16(first, D, monkeypatch, device_ok):

@@ -160,6 +160,21 @@ template <int BIAS>
 __device__ __forceinline__ float weight(float s, float m) {
   return ex2(kNatural<BIAS> ? (s - m) * kLog2e : s - m);
 }
+// How far a score may rise above the running maximum before that moves; and the power of two that all weights of a call, and
+// their sums with them, are multiplied with.  fp16 ends at 2^16 and its steps at 2^-24: with weights up to 2^8 a factor of 2^7 is
+// the most, and then a weight is kept, in its two terms, down to 2^-32 of the largest one and not to 2^-25 (65536 keys 17.9 below
+// one more, in 5 stretches: the share of the stretch with that one, 1/5 of what they add up to, was lost).  The range of bf16 is
+// that of fp32.
+template <int BIAS, typename T>
+constexpr float kRise = kNatural<BIAS> && !Pack2<T>::kIsBf16 ? 8 / kLog2e : 8;
+template <typename T>
+constexpr float kLift = Pack2<T>::kIsBf16 ? 0 : 7;
+template <int BIAS, typename T>
+__device__ __forceinline__ float lifted_weight(float s, float m) {
+  if constexpr (Pack2<T>::kIsBf16) return weight<BIAS>(s, m);
+  // (added to the difference: to m, which may be large, it would be rounded, to something else for each m)
+  return ex2(kNatural<BIAS> ? fmaf(s - m, kLog2e, kLift<T>) : s - m + kLift<T>);
+}
 // What a stretch with maximum m counts beside one with m_all >= m; 0 where it has no key (its sums are zero then, or NaN, which
 // stays).
 template <int BIAS>
@@ -709,7 +724,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
           }
           if (!(keys >> (k * 16 + r + 8 * (i >> 1)) & 1)) y = -INFINITY;
           s[g][k][i] = y;
-          need = need || y - mx[g][i & 1] > 8.f;  // (the difference that the weight is taken of: a sum may be rounded up by more)
+          need = need || y - mx[g][i & 1] > kRise<BIAS, T>;  // (the difference that the weight is taken of)
         }
     if (BIAS != 0 && info.y == 0) load_b(tile + 1, s_info[warp][place + 1 == S ? 0 : place + 1].x);
     if (__any_sync(0xffffffffu, need)) {
@@ -737,7 +752,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
       for (int k = 0; k < MB; ++k) {
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = weight<BIAS>(s[g][k][i], i & 1 ? m_1 : m_0);
+        for (int i = 0; i < 4; ++i) w[i] = lifted_weight<BIAS, T>(s[g][k][i], i & 1 ? m_1 : m_0);
         l[g][0] += w[0] + w[2];
         l[g][1] += w[1] + w[3];
 #pragma unroll
