@@ -29,6 +29,7 @@
 
 #include "fa_common.cuh"
 #include "fa_host.cuh"
+#include "fa_ring.h"
 
 namespace fa {
 
@@ -889,11 +890,15 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1) paged_kernel(const __grid_
     next_b = b + 1, next_tile = 0;
   }
   copies_landed();
-  if (s_abort)  // a copy never came: those that are still under way are waited for, within limits
+  if (s_abort) {  // a copy never came: those that are still under way are waited for in their order, all together 0.1 s at most
+    const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
-    for (int i = 0; i < S; ++i)
-      for (int spins = 0; spins < 4096 && !mbar_try_wait(&full[i], phase); ++spins) {
-      }
+    for (int j = 0; j < S; ++j) {
+      const int i = place + j < S ? place + j : place + j - S;
+      while (!mbar_try_wait(&full[i], ring_phase(i, place, phase)))
+        if (global_timer_ns() - t0 > 100000000ull) return;
+    }
+  }
 }
 
 // Joins the sums of the sequences that go on.  A team of threads, four values each, adds up sums of a slice of a (sequence, head);
