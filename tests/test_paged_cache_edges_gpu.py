@@ -1,5 +1,5 @@
-"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, weights far below the
-largest one, scores at the end of what fp32 tells apart."""
+"""GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, memory that a
+bias takes, weights far below the largest one, scores at the end of what fp32 tells apart."""
 import pytest
 import torch
 
@@ -97,6 +97,37 @@ def test_operators_refuse_what_would_lose_a_derivative(device_ok):
         want = fa.paged_attention_fn(q, kc, vc, table, n)
         assert torch.equal(fa.paged_attention_op(q.clone().requires_grad_(), kc, vc, table, n), want)
     assert torch.equal(fa.paged_attention_op(q, kc, vc, table, n), want)
+
+
+# ---------------------------------------------------------------------------------- biases that are converted
+@pytest.mark.parametrize("what", ["fp64 table", "fp16 a head", "fp64 a sequence", "fp32 every other", "mask every other", "one number"])
+def test_expanded_biases_are_not_written_out(what, device_ok):
+    """A bias that has to be converted, or laid out anew, and is expanded over the batch or the heads: a copy of what there is of
+    it, not of the (B, H, N) that it stands for."""
+    B, H, page, width = 12, 32, 16, 64
+    N = page * width
+    kc, vc, table, n = make_cache([700 - 50 * i for i in range(B)], page, 8, 64, BF, 64, width=width)
+    q = make_q(B, H, 64, BF, 64)
+    x = torch.randn(B, H, 2 * N, generator=torch.Generator().manual_seed(65)).to(HF).cuda()
+    bias = {"fp64 table": lambda: x[:1, :1, :N].double(), "fp16 a head": lambda: x[:1, :, :N].clone(),
+            "fp64 a sequence": lambda: x[:, :1, :N].double(), "fp32 every other": lambda: x[:1, :1].float()[:, :, ::2],
+            "mask every other": lambda: (x[:, :1] > 0)[:, :, ::2], "one number": lambda: x[:1, :1, :1].to(BF)}[what]().expand(B, H, N)
+    full = bias.contiguous()  # (as it is, or in fp32 for another dtype)
+    want = fa.paged_attention_fn(q, kc, vc, table, n, full if full.dtype in (torch.bool, BF) else full.float())
+    fa.paged_attention_fn(q, kc, vc, table, n)
+    torch.cuda.synchronize()
+
+    def peak(bias):
+        torch.cuda.reset_peak_memory_stats()
+        start = torch.cuda.memory_allocated()
+        out = fa.paged_attention_fn(q, kc, vc, table, n, bias)
+        return out, torch.cuda.max_memory_allocated() - start
+
+    plain = peak(None)[1]  # result and workspace
+    got, used = peak(bias)
+    assert torch.equal(got, want)
+    # at most one fp32 number an element of the largest of them, (1, H, N), in blocks of 512 bytes
+    assert used - plain <= 4 * H * N + 512
 
 
 # ---------------------------------------------------------------------------------- weights

@@ -561,6 +561,15 @@ Tensor rows_ready(const Tensor& t) {
   if (st[2] == 1 && (st[0] | st[1]) % 8 == 0 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }
+// A (B, H, N) bias as `dtype` with a unit inner stride.  Where that takes a copy, dimensions that are expanded stay so: a table by
+// position is written once, not for every head of every sequence.
+Tensor bias_rows_ready(const Tensor& bias, at::ScalarType dtype) {
+  if (bias.scalar_type() == dtype && bias.stride(2) == 1) return bias;
+  const Tensor base = bias.narrow(0, 0, bias.stride(0) == 0 ? 1 : bias.size(0)).narrow(1, 0, bias.stride(1) == 0 ? 1 : bias.size(1));
+  Tensor out = empty_on(bias, base.sizes(), dtype);
+  out.copy_(base);
+  return out.expand(bias.sizes());
+}
 Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 // What autograd compares to notice that a saved tensor was written to.
 void written(const Tensor& t) {
@@ -611,8 +620,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, cons
   if (bias.defined()) {
     const auto dt = bias.scalar_type();
     p.bias_kind = dt == at::kBool ? FA_BIAS_BOOL : dt == q.scalar_type() ? FA_BIAS_SAME : FA_BIAS_F32;
-    tb = p.bias_kind == FA_BIAS_F32 && dt != at::kFloat ? bias.to(at::kFloat) : bias;
-    if (tb.stride(2) != 1) tb = tb.contiguous();
+    tb = bias_rows_ready(bias, p.bias_kind == FA_BIAS_F32 ? at::kFloat : dt);
     p.bias = tb.const_data_ptr();
     p.bias_stride[0] = tb.stride(0), p.bias_stride[1] = tb.stride(1);
   }
