@@ -1,5 +1,5 @@
 """GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, memory that a
-bias takes, weights far below the largest one, scores at the end of what fp32 tells apart."""
+bias takes, rows of the cache itself, weights far below the largest one, scores at the end of what fp32 tells apart."""
 import pytest
 import torch
 
@@ -128,6 +128,38 @@ def test_expanded_biases_are_not_written_out(what, device_ok):
     assert torch.equal(got, want)
     # at most one fp32 number an element of the largest of them, (1, H, N), in blocks of 512 bytes
     assert used - plain <= 4 * H * N + 512
+
+
+# ---------------------------------------------------------------------------------- rows of the cache itself
+@pytest.mark.parametrize("Hkv,D,page", [(8, 128, 16), (1, 16, 7), (3, 256, 64)])
+@pytest.mark.parametrize("by", [1, -1, 0, 1000])
+def test_rows_that_lie_in_the_cache_are_moved_as_they_were(Hkv, D, page, by, device_ok):
+    """Rows read from slots that the same call writes: each slot gets what its source held before the call."""
+    pages = -(-5000 // page)
+    g = torch.Generator().manual_seed(66)
+    kc, vc = (torch.randn(pages, page, Hkv, D, generator=g).to(BF).cuda() for _ in range(2))
+    total = pages * page
+    src = torch.arange(total)
+    slots = (src + by) % total if by >= 0 else src + by  # (one of them then has no slot)
+    want_k, want_v = kc.clone(), vc.clone()
+    has = slots >= 0
+    # k out of the values and v out of the keys
+    want_k.view(total, Hkv, D)[slots[has].cuda()] = vc.view(total, Hkv, D)[src[has].cuda()]
+    want_v.view(total, Hkv, D)[slots[has].cuda()] = kc.view(total, Hkv, D)[src[has].cuda()]
+    fa.paged_kv_write(vc.view(total, Hkv, D), kc.view(total, Hkv, D), kc, vc, slots.cuda())
+    assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
+
+
+def test_a_page_is_copied_to_another_one(device_ok):
+    kc, vc, table, n = make_cache([48], 16, 2, 64, HF, 67, stale=0.0)
+    to = next(i for i in range(kc.shape[0]) if i not in table[0].tolist())
+    fa.paged_kv_write(kc[table[0, 1]], vc[table[0, 1]], kc, vc, torch.arange(to * 16, to * 16 + 16, device="cuda"))
+    assert torch.equal(kc[to], kc[table[0, 1]]) and torch.equal(vc[to], vc[table[0, 1]])
+    q = make_q(1, 4, 64, HF, 67)
+    want = fa.paged_attention_fn(q, kc, vc, table, n)
+    fork = table.clone()
+    fork[0, 1] = to
+    assert torch.equal(fa.paged_attention_fn(q, kc, vc, fork, n), want)
 
 
 # ---------------------------------------------------------------------------------- weights

@@ -561,6 +561,17 @@ Tensor rows_ready(const Tensor& t) {
   if (st[2] == 1 && (st[0] | st[1]) % 8 == 0 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }
+// The memory from the first to the last element of a tensor.
+struct Extent {
+  const char *begin, *end;
+  explicit Extent(const Tensor& t) : begin(static_cast<const char*>(t.const_data_ptr())) {
+    const auto size = t.sizes(), stride = t.strides();
+    int64_t last = 0;
+    for (size_t i = 0; i < size.size(); ++i) last += (size[i] - 1) * stride[i];
+    end = begin + (last + 1) * static_cast<int64_t>(t.element_size());
+  }
+  bool meets(const Extent& x) const { return begin < x.end && x.begin < end; }
+};
 // A (B, H, N) bias as `dtype` with a unit inner stride.  Where that takes a copy, dimensions that are expanded stay so: a table by
 // position is written once, not for every head of every sequence.
 Tensor bias_rows_ready(const Tensor& bias, at::ScalarType dtype) {
@@ -669,7 +680,12 @@ void paged_kv_write(const Tensor& k, const Tensor& v, const Tensor& kc, const Te
   at::AutoDispatchBelowADInplaceOrView below;
   raise_if_unhealthy(device);
   if (T == 0) return;
-  const Tensor tk = rows_ready(k), tv = rows_ready(v), ts = dense(slots);
+  const Extent k_room(kc), v_room(vc);
+  const auto apart = [&](Tensor rows) {  // (what is read must not be written at the same time)
+    const Extent x(rows);
+    return x.meets(k_room) || x.meets(v_room) ? rows.clone(at::MemoryFormat::Contiguous) : rows;
+  };
+  const Tensor tk = apart(rows_ready(k)), tv = apart(rows_ready(v)), ts = dense(slots);
   fa_kv_write_params p{};
   p.struct_size = sizeof(fa_kv_write_params);
   p.device = device;

@@ -45,7 +45,9 @@ def paged_attention_fn(q, k_cache, v_cache, block_table, seq_lens, bias=None, sm
 def paged_kv_write(k, v, k_cache, v_cache, slot_mapping) -> None:
     """Writes k, v (T, Hkv, D) into the caches (pages, page_size, Hkv, D), token t into row slot % page_size of page
     slot // page_size with slot = slot_mapping[t] (int64).  Tokens with a slot below 0 or behind the cache are not written.  The
-    slots of a call must differ from one another: of two tokens with one slot, parts of both may stay."""
+    slots of a call must differ from one another: of two tokens with one slot, parts of both may stay.  Rows of the cache itself
+    can be given (a page copied to another, tokens moved): they are copied first, so each slot gets what was there before the
+    call."""
     _native.paged_kv_write(k, v, k_cache, v_cache, slot_mapping)
 
 
