@@ -1,10 +1,12 @@
 """GPU tests of the paged cache at its edges: what a bias of -inf leaves out, calls that want a derivative, memory that a
-bias takes, rows of the cache itself, weights far below the largest one, scores at the end of what fp32 tells apart."""
+bias takes, rows of the cache itself, weights far below the largest one, scores at the end of what fp32 tells apart,
+sequences that are not split."""
 import pytest
 import torch
 
 import triton_flashattn_b200 as fa
 from tests.test_paged_cache_gpu import BF, HF, INF, check, make_cache, make_q
+from triton_flashattn_b200 import _cabi
 
 pytestmark = pytest.mark.gpu
 
@@ -222,3 +224,27 @@ def test_scores_so_large_that_fp32_steps_by_16(first, D, monkeypatch, device_ok)
     pos = torch.arange(table.shape[1] * 16, device="cuda")
     bias = (first + 16.0 * (pos // 32 % 2)).float().expand(1, 3, -1)
     check(fa.paged_attention_fn(q, kc, vc, table, n, bias), q, kc, vc, table, n, bias)
+
+
+# ---------------------------------------------------------------------------------- sequences that are not split
+@pytest.mark.parametrize("B,width,Hkv,group,D,launches", [
+    (1, 1, 2, 16, 256, 1), (40, 1, 2, 16, 256, 1), (700, 1, 1, 12, 256, 1),  # one tile: nothing to split, whatever the warps share
+    (1, 2, 1, 1, 64, 1), (300, 2, 3, 2, 32, 1), (5, 1, 1, 20, 128, 1), (33, 1, 5, 1, 128, 1),
+    (200, 4, 8, 2, 128, 1), (200, 3, 12, 1, 64, 1),  # as many sequences as CTAs, a unit for each warp
+    (1, 3, 8, 4, 128, 2), (147, 4, 8, 2, 128, 2), (200, 4, 2, 16, 256, 2), (200, 5, 8, 2, 128, 2)])
+def test_sequences_that_are_not_split(B, width, Hkv, group, D, launches, device_ok):
+    """One launch where no sequence can be split or none has to be, else two; pages that are not there among them."""
+    lib = _cabi.load()
+    g = torch.Generator().manual_seed(72)
+    lens = torch.randint(0, width * 16 + 1, (B,), generator=g).tolist()
+    lens[0] = width * 16
+    for dtype in (BF, HF):
+        kc, vc, table, n = make_cache(lens, 16, Hkv, D, dtype, 73, width=width)
+        if B > 3:
+            table[2, 0] = -1
+        q = make_q(B, Hkv * group, D, dtype, 73)
+        before = lib.fa_launch_count()
+        out = fa.paged_attention_fn(q, kc, vc, table, n)
+        if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+            assert lib.fa_launch_count() - before == launches
+        check(out, q, kc, vc, table, n)

@@ -5,8 +5,15 @@
 namespace fa {
 namespace {
 
-// Sequences of at most this many keys are not split over CTAs: one launch less.  Whole / split, us: one of 48 keys 7.0 / 6.7, 64 of up
-// to 48 9.4 / 10.3; one of 96 9.6 / 6.9, 64 of up to 100 13.1 / 13.9.
+// Where no sequence is split over CTAs, there is one launch less.  Sequences of one tile cannot be.  Those of up to so many keys are not
+// where there are as many of them as CTAs and a CTA's warps all have a unit of their own.  Whole / split, us, up to 64 keys
+// each (bf16; 8 key heads of 128 with 4 heads, 12 of 64 with one, 2 of 256 with 16):
+//     1 sequence       8.1 / 7.1    10.1 / 10.0   11.6 / 9.1
+//    64 sequences     11.8 / 12.8   12.8 / 12.2   15.2 / 14.6
+//   148 sequences     14.5 / 18.1   17.2 / 17.2   19.8 / 22.7
+//  2048 sequences     70.7 / 73.0   82.2 / 83.5   93.6 / 68.0 (two units, four warps: half of them idle when whole)
+// and up to 128 keys, 512 sequences: 39.1 / 39.2, 42.6 / 39.7, 48.7 / 41.2.  One tile (16 keys), 1 sequence: 5.5 / 6.3, 7.9 / 8.9,
+// 7.3 / 8.2.
 constexpr int kWholeKeys = 64;
 
 PagedPlan plan_paged(const fa_paged_params& p) {
@@ -43,8 +50,7 @@ PagedPlan plan_paged(const fa_paged_params& p) {
   const int64_t most_ctas = p.B * ((cap + keys - 1) / keys);
   const int sms = persistent_grid(1 << 30);
   x.ctas = static_cast<int>(most_ctas < sms ? most_ctas : sms);
-  x.whole = cap <= kWholeKeys;
-  if (x.whole) x.parts = 1;
+  x.whole = cap <= keys || (cap <= kWholeKeys && x.parts == 1 && p.B >= sms);
   const int stretches = x.ctas * x.parts;
   x.by_seq = p.B <= kFew || p.B <= stretches;
   x.joints = x.by_seq ? p.B : stretches;
