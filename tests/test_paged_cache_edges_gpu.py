@@ -230,8 +230,9 @@ def test_scores_so_large_that_fp32_steps_by_16(first, D, monkeypatch, device_ok)
 @pytest.mark.parametrize("B,width,Hkv,group,D,launches", [
     (1, 1, 2, 16, 256, 1), (40, 1, 2, 16, 256, 1), (700, 1, 1, 12, 256, 1),  # one tile: nothing to split, whatever the warps share
     (1, 2, 1, 1, 64, 1), (300, 2, 3, 2, 32, 1), (5, 1, 1, 20, 128, 1), (33, 1, 5, 1, 128, 1),
-    (200, 4, 8, 2, 128, 1), (200, 3, 12, 1, 64, 1),  # as many sequences as CTAs, a unit for each warp
-    (1, 3, 8, 4, 128, 2), (147, 4, 8, 2, 128, 2), (200, 4, 2, 16, 256, 2), (200, 5, 8, 2, 128, 2)])
+    (200, 4, 8, 2, 128, 1), (1, 3, 8, 4, 128, 1), (147, 4, 12, 1, 64, 1),  # up to 64 keys, a unit for each warp
+    (140, 4, 2, 16, 256, 1), (1, 4, 1, 8, 128, 1),  # or no more sequences than CTAs
+    (200, 4, 2, 16, 256, 2), (200, 3, 1, 8, 128, 2), (200, 5, 8, 2, 128, 2)])
 def test_sequences_that_are_not_split(B, width, Hkv, group, D, launches, device_ok):
     """One launch where no sequence can be split or none has to be, else two; pages that are not there among them."""
     lib = _cabi.load()

@@ -5,15 +5,16 @@
 namespace fa {
 namespace {
 
-// Where no sequence is split over CTAs, there is one launch less.  Sequences of one tile cannot be.  Those of up to so many keys are not
-// where there are as many of them as CTAs and a CTA's warps all have a unit of their own.  Whole / split, us, up to 64 keys
-// each (bf16; 8 key heads of 128 with 4 heads, 12 of 64 with one, 2 of 256 with 16):
-//     1 sequence       8.1 / 7.1    10.1 / 10.0   11.6 / 9.1
-//    64 sequences     11.8 / 12.8   12.8 / 12.2   15.2 / 14.6
-//   148 sequences     14.5 / 18.1   17.2 / 17.2   19.8 / 22.7
-//  2048 sequences     70.7 / 73.0   82.2 / 83.5   93.6 / 68.0 (two units, four warps: half of them idle when whole)
-// and up to 128 keys, 512 sequences: 39.1 / 39.2, 42.6 / 39.7, 48.7 / 41.2.  One tile (16 keys), 1 sequence: 5.5 / 6.3, 7.9 / 8.9,
-// 7.3 / 8.2.
+// Where no sequence is split over CTAs, there is one launch less.  Sequences of one tile cannot be.  Those of up to so many keys are
+// not, unless that leaves warps idle (they have no parts of a stretch then) and there are more sequences than CTAs.  Whole / split,
+// us, bf16, tables of 64 keys (8 key heads of 128 with 4 heads; 1 of 128 with 8; 12 of 64 with 1; 2 of 256 with 16):
+//     1 sequence,  17 keys      6.5 / 7.3      5.7 / 7.1      7.9 / 8.9      8.7 / 8.8
+//                  64           8.2 / 7.1      7.3 / 6.9     10.1 / 9.9     11.6 / 9.1
+//    64 sequences, 17           9.1 / 10.6     8.1 / 9.6     10.4 / 10.2    11.0 / 13.9
+//                  64          11.4 / 12.7     9.7 / 10.1    13.0 / 14.0    13.9 / 16.4
+//   148 sequences, 64          14.1 / 15.9     9.8 / 10.0    14.0 / 14.2    15.9 / 22.6
+//  1000 sequences, 64          55.0 / 57.8    37.0 / 21.6    51.0 / 52.2    62.8 / 53.0   (warps 8 of 8, 1 of 8, all, 2 of 4)
+// and tables of 128, full: 1 sequence 11.8 / 7.5, 148 of up to 128 keys 19.9 / 21.6.
 constexpr int kWholeKeys = 64;
 
 PagedPlan plan_paged(const fa_paged_params& p) {
@@ -50,7 +51,8 @@ PagedPlan plan_paged(const fa_paged_params& p) {
   const int64_t most_ctas = p.B * ((cap + keys - 1) / keys);
   const int sms = persistent_grid(1 << 30);
   x.ctas = static_cast<int>(most_ctas < sms ? most_ctas : sms);
-  x.whole = cap <= keys || (cap <= kWholeKeys && x.parts == 1 && p.B >= sms);
+  x.whole = cap <= keys || (cap <= kWholeKeys && (x.parts == 1 || p.B <= sms));
+  if (x.whole && cap > keys) x.parts = 1;
   const int stretches = x.ctas * x.parts;
   x.by_seq = p.B <= kFew || p.B <= stretches;
   x.joints = x.by_seq ? p.B : stretches;
