@@ -304,7 +304,8 @@ int fa_kv_write(const fa_kv_write_params* p, void* stream);
  *   pages come off the top of the stack into block_table, lens_out[b] is its new length, and slots[row] the slot of each of its
  *   tokens; all other slots are -1, and lens_out[b] of a request that got nothing is lens[b].  count_out: pages left.
  * fa_kv_release: the pages of each request b with finished[b] != 0 go back on the stack, requests and pages in order, and
- *   lens_out[b] is 0 (else lens[b]).  Pages beyond the stack's capacity are dropped.  block_table is only read.
+ *   lens_out[b] is 0 (else lens[b]).  Pages beyond the stack's capacity are dropped.  block_table is only read.  What goes back is
+ *   not looked at: lengths and table are what fa_kv_extend made them and no page is in two finished rows, or it is given out twice.
  *
  * lens_out may be lens, and count_out may be count.
  */

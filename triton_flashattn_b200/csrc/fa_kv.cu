@@ -84,8 +84,10 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WritePara
 // shared out over their warps, a run of neighbours each, so that a lane looks for the request of its first one, and again only
 // where its next one is another's.  Where lens_out is lens or count_out is count, the CTAs are one cluster, with a barrier between
 // looking and writing.
-// What bounds a call is latency: a launch, the lengths, the pages, the stores.  256 requests with a token each 4.8 us; prompts of 131 k
-// tokens 8.4 (40 with a search for each token and a cluster in any case); 131 k pages given back 5.4 (26).
+// What bounds a call is latency: a launch, the lengths, the pages, the stores.  us in a captured graph, results apart / in place:
+// 256 requests with a token each 5.1 / 5.1; prompts of 131 k tokens 7.1 / 18.0 (40 with a search for each token), of 1 M 17.7 / 97;
+// 7 of 256 requests released 3.1 / 3.7, 131 k pages given back 5.3 / 12.7 (26).  In place, long lists wait for 8 CTAs where apart
+// there are up to 64.
 constexpr int kThreads = 512;
 
 struct TableParams {

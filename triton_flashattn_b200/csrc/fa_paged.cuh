@@ -8,8 +8,12 @@
 // shares it), so it is a stream from memory.  Each warp has a ring of tiles of 16 or 32 keys in shared memory that it fills itself,
 // by tile copies where pages are whole boxes of 8 or 16 keys and else 16 bytes a lane, and empties with the warp-level matrix
 // instruction: the heads that share a key head are the 8 or 16 columns of the product.  Its copies run ahead over the ends of
-// sequences and heads, so the stream does not stop there.  (tcgen05 would want 128 rows of queries where there are 4 or 8, and
-// a hand-off between warps for every tile; a tile's 40 products take a tenth of the time that its bytes do.)
+// sequences and heads, so the stream does not stop there.
+//   tcgen05 would take the same products: 128 keys, or 128 elements of a value, as rows and 16 queries as columns.  Where the
+// memory is the bound it has nothing to give (a tile's 32 products, at head dim 128 with up to 8 heads, keep the tensor pipe busy for a
+// fifth of the time) and costs tiles of 128 keys and hand-offs between warps for each.  With 16 heads of 256 there are four warps,
+// one a scheduler, each ready to issue in 15 % of the cycles: there the latency inside a tile is the bound, and tcgen05, or two
+// warps a ring, could help.  Neither is built.
 //
 // Lengths are on the device and differ, and one long sequence must fill the SMs as well as thousands of short ones: the tiles of
 // all sequences, in order, are one line, and each CTA takes an equal stretch of it with all key heads, a warp one head (or one

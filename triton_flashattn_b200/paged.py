@@ -31,7 +31,8 @@ def paged_attention_fn(q, k_cache, v_cache, block_table, seq_lens, bias=None, sm
     block_table       (B, W) int32: the key at position n lies in row n % page_size of page block_table[b, n // page_size]
     seq_lens          (B,) int32: keys of each sequence, the new token's own among them (write it first)
     bias              (B, H, W * page_size), as in `flash_attention_fn`: bool (False is left out) or float (added to the scaled
-                      scores); expanded views are read in place, other float dtypes than q's as fp32
+                      scores); expanded views are read in place, other float dtypes than q's as fp32 (converted, fp32 itself
+                      apart, and so are other inner strides copied: what there is of an expanded view)
     sm_scale          None: 1 / sqrt(D)
 
     A sequence of length 0 and a row whose mask leaves nothing give 0.  What a mask or a bias of -inf leaves out takes no part,
@@ -71,8 +72,11 @@ def paged_kv_extend(block_table, seq_lens, new_lens, free_pages, free_count, pag
 def paged_kv_release(block_table, seq_lens, finished, free_pages, free_count, page_size: int,
                      inplace: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """Puts the pages of the requests with finished[b] (bool) back on the stack, in order, in place in free_pages; returns
-    (seq_lens after, 0 for the finished; free_count after).  The table is only read.  No two finished requests may hold the
-    same page."""
+    (seq_lens after, 0 for the finished; free_count after).  The table is only read.
+
+    Lengths and table of a finished request must be what `paged_kv_extend` made them, and no two finished requests may hold the
+    same page: what goes back is not looked at, and a page that is on the stack twice, or was never taken from it, is given to two
+    requests later on."""
     return _native.paged_kv_release(block_table, seq_lens, finished, free_pages, free_count, page_size, inplace)
 
 
